@@ -216,6 +216,112 @@ int l2_decode_greedy(l2_model *m, l2_state *s, int32_t token, int32_t pos, int32
 int l2_generate_greedy(l2_model *m, l2_state *s, const int32_t *prompt, int n_prompt, int steps,
                        int use_prefill, int32_t *out_ids, int *n_out, double *ms);
 
+/* ---- a cache in pages, for programs with a loop of their own --------------- */
+
+/* No counterpart in the reference, whose cache is one array per RunState (src/models.rs:29-42).  A pool holds keys and values of many
+ * sequences for all layers, in pages of page_size positions that the caller deals out: which page holds which positions of a sequence is
+ * in a table that comes with each call.  The operators below work on DEVICE pointers: they enqueue kernels on hip_stream (a
+ * hipStream_t; NULL is the default stream) and return without waiting; they allocate nothing, and may be made while hip_stream is
+ * captured into a graph, which holds kernels only.  Calls on one pool may overlap in time as far as they neither write what another
+ * reads nor share a workspace.  A pool is used on the device it was created on (current there, and the stream's). */
+typedef struct l2_kvpool l2_kvpool;
+
+/* Types of the callers' rows and logits. */
+enum { L2_F32 = 0, L2_F16 = 1, L2_BF16 = 2 };
+
+/* What a pool holds of a value x of a row (the head_size values of one position and kv head).  Eight bits: a code c and one fp32 scale s per
+ * row, with a = max |x| over the row;
+ *   L2_KV_I8:   s = a / 127, c = the whole number nearest to x / s
+ *   L2_KV_E4M3: s = a / 448, c = the float of four exponent and three mantissa bits nearest to x / s
+ * the quotient a / 127 (448) rounded to fp32 and c from the exact quotient x / s, ties to even; the row stands for c * s.  Rows with
+ * a < 2^-60 are held as zeros; rows with a value that is not finite are NaN throughout.  Sixteen bits: x rounded to nearest. */
+enum { L2_KV_I8 = 0, L2_KV_E4M3 = 1, L2_KV_F16 = 2, L2_KV_BF16 = 3 };
+
+/* page_size 16, 32, 64, 128 or 256; head_size 64 or 128; kv heads up to 65535.  Zero-filled device memory:
+ * 2 * n_layers * n_pages * page_size * n_kv_heads * (head_size * (1 or 2 bytes) + 4 for 8 bits).  Creating a pool also does what first
+ * launches of all operators here do besides enqueueing (l2_sample_device included), on the device that is current. */
+int l2_kvpool_create(int n_layers, int n_pages, int page_size, int n_kv_heads, int head_size, int kv_type, l2_kvpool **out);
+void l2_kvpool_free(l2_kvpool *p); /* waits for the device */
+size_t l2_kvpool_bytes(const l2_kvpool *p);
+
+/* The sequences of a call.  starts, lengths and pages are device arrays, read when the kernels run; the numbers are limits that hold for
+ * everything they may contain at that time (a captured call is replayed with other contents): sequence i has the rows
+ * [starts[i], starts[i+1]) of the call's arrays, which are its last positions, up to lengths[i] - 1; position t of it lies in slot
+ * t % page_size of page pages[i * max_pages + t / page_size].  A sequence may have no rows, or no positions; rows before starts[0]
+ * and behind starts[n_seqs] are left as they are.  Entries of pages that no row has to do with are not read, and one outside
+ * 0..n_pages-1 is no page: what it would hold is not there.  Contents beyond the limits are cut off at them: the values of such a sequence are then
+ * unspecified, but nothing outside the arrays and the pool is touched. */
+typedef struct l2_kvbatch {
+    const int32_t *starts;  /* [n_seqs + 1], ascending */
+    const int32_t *lengths; /* [n_seqs]: positions of the sequence, its rows here included */
+    const int32_t *pages;   /* [n_seqs][max_pages] */
+    int32_t n_seqs;         /* up to 65535 */
+    int32_t max_pages;
+    int32_t n_rows;     /* rows of the call's arrays */
+    int32_t max_rows;   /* the most rows of a sequence */
+    int32_t max_length; /* the most positions of a sequence */
+} l2_kvbatch;
+
+/* Writes rows into one layer: k_dev and v_dev of `type`, [n_rows][n_kv_heads][head_size] with k_stride and v_stride elements from row to
+ * row (0: dense).  A slot that two rows of a call name holds a mixture of them.  Aligned as their type is. */
+int l2_kvpool_write(l2_kvpool *p, int layer, const l2_kvbatch *batch, const void *k_dev, const void *v_dev, int type, int64_t k_stride,
+                    int64_t v_stride, void *hip_stream);
+
+/* The inverse: what the pool holds at the rows' positions, c * s rounded to fp32 and then to `type`.  A row without a page, or of a position
+ * below zero, reads as zeros. */
+int l2_kvpool_read(l2_kvpool *p, int layer, const l2_kvbatch *batch, void *k_dev, void *v_dev, int type, int64_t k_stride,
+                   int64_t v_stride, void *hip_stream);
+
+/* Attention of the rows over one layer: q_dev and out_dev of `type`, [n_rows][n_heads][head_size], n_heads a multiple of the pool's (query
+ * head h reads kv head h / (n_heads / n_kv_heads)); out may be q.  The row of position pos sees the positions t <= pos that have a page, with a window > 0
+ * only those of the last `window` (t > pos - window) and of the first `sinks`.  out = sum over t of softmax(scale * q.k_t) v_t;
+ * zeros where nothing is seen.  Keys and values come from the pool, those of the rows included (l2_kvpool_write first).  Scores, statistics and sums
+ * are fp32; q and the softmax's weights enter the matrix cores as one 16-bit number each for 16-bit rows and as several, to within 2^-22,
+ * for fp32 rows.  What is not seen has no influence, NaN and infinities included. */
+typedef struct l2_attention {
+    int32_t n_heads;
+    int32_t type;       /* L2_F32, L2_F16 or L2_BF16 */
+    float scale;        /* above zero; 0: 1 / sqrt(head_size) */
+    int32_t window;     /* 0: none */
+    int32_t sinks;
+    int64_t q_stride;   /* elements from row to row; 0: dense */
+    int64_t out_stride;
+} l2_attention;
+/* Bytes of device memory that such a call wants as its workspace (aligned to 16; its contents do not matter before the call and mean nothing
+ * behind it).  They follow from the limits in `batch`, not from its arrays.  May be 0. */
+int l2_kvpool_attention_workspace(const l2_kvpool *p, const l2_kvbatch *batch, const l2_attention *a, size_t *bytes);
+int l2_kvpool_attention(l2_kvpool *p, int layer, const l2_kvbatch *batch, const l2_attention *a, const void *q_dev, void *out_dev,
+                        void *workspace_dev, size_t workspace_bytes, void *hip_stream);
+
+/* ---- sampling on the device ------------------------------------------------- */
+
+/* One token id per row of logits_dev (`type`, [rows][vocab], `stride` elements from row to row, 0: dense), from a random number u in [0, 1) that the
+ * caller gives for each row, as Random::random (src/util.rs:79-82) makes them.  With the tokens in falling order of their logits l, the lower id
+ * first among equals, and weights w = exp((l - max l) / temperature):
+ *   top_k:  the first top_k tokens are kept            (off: <= 0)
+ *   top_p:  of these, the fewest from the front whose weights reach top_p of the sum of these    (off: >= 1)
+ *   min_p:  of these, those with w >= min_p (of the largest weight, which is 1)               (off: <= 0)
+ * The first is always kept.  The answer is the first id, in the vocabulary's order, at which the running sum of the kept weights passes u times
+ * their sum (Random::sample, src/util.rs:102-113).  A temperature of 0 (or below, or NaN) takes the first token.  Weights are whole multiples of 2^-44 and sums of them
+ * exact, so a row's answer is the same in every batch and call.  NaN logits count as -infinity; a row with nothing else gets -1.  An infinite
+ * logit shares everything with its equals.  vocab up to 2^19.  ids_dev is host-visible or device memory.
+ * Enqueued on hip_stream without waiting; allocates nothing; may be captured (after a first call, or l2_kvpool_create, on the device).
+ * temperature, top_k, top_p, min_p and u are device arrays [rows]; any of the first four may be NULL: 1, off, off, off. */
+typedef struct l2_sampling {
+    const float *temperature;
+    const int32_t *top_k;
+    const float *top_p;
+    const float *min_p;
+    const float *u;
+} l2_sampling;
+int l2_sample_device(const void *logits_dev, int type, int rows, int vocab, int64_t stride, const l2_sampling *s, int32_t *ids_dev,
+                     void *hip_stream);
+
+/* l2_decode_greedy with that choice in the place of the argmax: forward, then one token from the logits, of which only the id comes back.
+ * L2_ERR_RANGE if no logit is a number above -infinity. */
+int l2_decode_sample(l2_model *m, l2_state *s, int32_t token, int32_t pos, float temperature, int32_t top_k, float top_p, float min_p,
+                     float u, int32_t *next);
+
 /* ---- text surface: tokenizer, Random, generate on strings ----------------- */
 
 typedef struct l2_tokenizer l2_tokenizer; /* Tokenizer (src/tokenizer.rs:13-19) */

@@ -33,8 +33,12 @@ SOURCES = {
     # the block kernels keep the reference's rounded-multiply-then-add where they restate it
     "kernels_misc.hip": ["-ffp-contract=off"],
     "kernels_attn.hip": ["-ffp-contract=off"],
+    "kernels_kvpool.hip": ["-ffp-contract=off"],
+    "kernels_kvattn.hip": ["-ffp-contract=off"],
+    "kernels_sample.hip": ["-ffp-contract=off"],
     "host.cpp": ["-x", "hip", "-ffp-contract=off"],
     "textgen.cpp": ["-x", "hip", "-ffp-contract=off"],
+    "host_kvpool.cpp": ["-x", "hip", "-ffp-contract=off"],
 }
 
 

@@ -479,6 +479,7 @@ AtWork::~AtWork() {
     device_calls.leave(device);
 }
 AtWork::AtWork(l2_model *m) : AtWork(m->device, &m->work) {}
+void l2_pass_by(int device) { device_calls.pass_by(device); }
 
 struct StepGraph {
     hipGraph_t graph = nullptr;
@@ -2430,6 +2431,28 @@ extern "C" int l2_decode_greedy(l2_model *m, l2_state *s, int32_t token, int32_t
     L2_TRY(check_tokens(m, &token, &pos, 1, &max_pos));
     L2_TRY(ensure_batch(m, 1));
     return steps_run(m, s, token, pos, 1, nullptr, 0, next);
+}
+
+extern "C" int l2_decode_sample(l2_model *m, l2_state *s, int32_t token, int32_t pos, float temperature, int32_t top_k, float top_p,
+                                float min_p, float u, int32_t *next) {
+    if (!m || !s || !next) return l2_fail(L2_ERR_ARG, "null argument");
+    if (s->m != m) return l2_fail(L2_ERR_ARG, "state belongs to another model");
+    const AtWork at_work(m);
+    int max_pos = 0;
+    L2_TRY(check_tokens(m, &token, &pos, 1, &max_pos));
+    L2_TRY(ensure_batch(m, 1));
+    ForwardIn in;
+    in.src.token = token, in.logits = m->logits, in.amax = m->amax, in.whole = true;
+    SampleSettings how{};
+    how.temperature0 = temperature, how.top_k0 = top_k, how.top_p0 = top_p, how.min_p0 = min_p, how.u0 = u;
+    L2_TRY(token_tries(m, [&]() -> int {
+        L2_TRY(forward_enqueue(m, s, 1, pos, in));
+        L2_TRY(sample_launch(m->logits, L2_F32, 1, m->d.vocab_size, m->d.vocab_size, how, m->hs.ids, m->stream));
+        return wait_host(m, nullptr, nullptr);
+    }));
+    if (m->hs.ids[0] < 0) return l2_fail(L2_ERR_RANGE, "sampling: no logit is a number above -infinity");
+    *next = m->hs.ids[0];
+    return L2_OK;
 }
 
 static int ensure_loop_buffers(l2_model *m, int n_prompt, int n_out) {

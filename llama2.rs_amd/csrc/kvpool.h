@@ -1,0 +1,98 @@
+// The pages of a pool and the sequences of a call, as the kernels on them see these (kernels_kvpool.hip, kernels_kvattn.hip).
+#pragma once
+
+#include <hip/hip_fp16.h>
+
+#include "l2_internal.h"
+
+// One layer of a pool.  Keys lie as [page][kv head][slot][value] and values as [page][kv head][value][slot]: both are then what the matrix
+// instructions of scores and of weighted sums want of their first operand, 16 contiguous bytes of the inner dimension per lane, without a transposition.
+// Scales lie as [page][kv head][slot].
+struct KvLayer {
+    void *k, *v;
+    float *k_scale, *v_scale; // 8 bits only
+    int n_pages, n_heads, head_size;
+    int page_shift; // log2 of the positions of a page
+};
+
+struct KvRows { // rows of the caller's: [row][kv head][value]
+    const void *k, *v;
+    int64_t k_stride, v_stride;
+    int type;
+};
+
+int kv_write_launch(const KvLayer &l, int kv_type, const l2_kvbatch &b, const KvRows &rows, hipStream_t st);
+int kv_read_launch(const KvLayer &l, int kv_type, const l2_kvbatch &b, const KvRows &rows, hipStream_t st);
+// Loads what the launches above need, on the current device.
+int kv_rows_warm_up();
+
+struct KvAttention {
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride;
+    int n_heads, type;
+    float scale;
+    int window, sinks;
+};
+// How the limits of a call are cut up: a function of them alone.
+struct KvAttnPlan {
+    size_t workspace; // bytes
+};
+void kv_attention_plan(const KvLayer &l, int kv_type, const l2_kvbatch &b, const KvAttention &a, KvAttnPlan *plan);
+int kv_attention_launch(const KvLayer &l, int kv_type, const l2_kvbatch &b, const KvAttention &a, const KvAttnPlan &plan, void *workspace,
+                        hipStream_t st);
+int kv_attention_warm_up();
+int sample_warm_up();
+
+#if defined(__HIPCC__)
+namespace kv {
+
+// What a call's arrays say of a sequence, cut off at the call's limits.
+struct Seq {
+    int first, rows; // rows of the call's arrays
+    int length;      // positions
+};
+__device__ __forceinline__ Seq sequence(const l2_kvbatch &b, int i) {
+    const int s0 = min(max(b.starts[i], 0), b.n_rows), s1 = min(max(b.starts[i + 1], s0), b.n_rows);
+    const int most = (int)min((int64_t)b.max_length, (int64_t)b.max_pages << 8);
+    return {s0, min(s1 - s0, b.max_rows), min(max(b.lengths[i], 0), most)};
+}
+
+// The sequence that a row of the call's arrays belongs to; n_seqs if none.
+__device__ __forceinline__ int sequence_of(const l2_kvbatch &b, int row) {
+    int lo = 0, hi = b.n_seqs; // the first i with starts[i + 1] > row
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (b.starts[mid + 1] > row) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo < b.n_seqs && b.starts[lo] <= row ? lo : b.n_seqs;
+}
+
+// The page of a position (in units of pages) of sequence i; -1: none.
+__device__ __forceinline__ int page_at(const l2_kvbatch &b, int n_pages, int i, int at) {
+    if (at >= b.max_pages) return -1;
+    const int p = b.pages[(int64_t)i * b.max_pages + at];
+    return (uint32_t)p < (uint32_t)n_pages ? p : -1;
+}
+
+// e4m3's codes from a float inside +-448 and back.
+__device__ __forceinline__ uint8_t to_e4m3(float y) { return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false); }
+__device__ __forceinline__ float from_e4m3(uint8_t c) { return __builtin_amdgcn_cvt_f32_fp8((int)c, 0); }
+
+__device__ __forceinline__ float bf16_float(uint16_t v) { return __builtin_bit_cast(float, (uint32_t)v << 16); }
+__device__ __forceinline__ uint16_t float_bf16(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
+
+__device__ __forceinline__ float load(const void *p, int type, int64_t i) {
+    if (type == L2_F32) return ((const float *)p)[i];
+    if (type == L2_F16) return (float)((const _Float16 *)p)[i];
+    return bf16_float(((const uint16_t *)p)[i]);
+}
+__device__ __forceinline__ void store(void *p, int type, int64_t i, float v) {
+    if (type == L2_F32) ((float *)p)[i] = v;
+    else if (type == L2_F16) ((_Float16 *)p)[i] = (_Float16)v;
+    else ((uint16_t *)p)[i] = float_bf16(v);
+}
+
+} // namespace kv
+#endif

@@ -344,6 +344,17 @@ int embed_launch(float *x, const float *emb, const TokenSource &src, int dim, in
 // two floats that another faithful expf may round it the other way, w[i] = d_i and bit i of `redo` is set.
 int sample_weights_launch(float *w, unsigned long long *redo, const float *logits, int n, float temperature,
                           const unsigned long long *amax, hipStream_t st);
+// One token per row of logits, as l2_sample_device describes; a null array stands for the value beside it.
+struct SampleSettings {
+    const float *temperature, *top_p, *min_p, *u;
+    const int32_t *top_k;
+    float temperature0, top_p0, min_p0, u0;
+    int32_t top_k0;
+};
+constexpr int kMaxVocab = 1 << 19; // weights up to 2^44: sums of them fit 64 bits
+int sample_launch(const void *logits, int type, int rows, int vocab, int64_t stride, const SampleSettings &s, int32_t *ids, hipStream_t st);
+// Work that is enqueued on a stream of the caller's and not waited for: steps of models on the device go out as launches of their own for a while.
+void l2_pass_by(int device);
 // *id = the index of the running maximum.
 int index_launch(const unsigned long long *amax, int32_t *id, hipStream_t st);
 // dst = src, n floats; for pieces of pinned host memory up to a megabyte: quicker than the copy engine, behind which a kernel starts

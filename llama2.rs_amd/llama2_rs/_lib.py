@@ -18,6 +18,8 @@ ERR_NAMES = {-1: "L2_ERR_ARG", -2: "L2_ERR_IO", -3: "L2_ERR_FORMAT", -4: "L2_ERR
 
 WQ, WK, WV, WO, W1, W2, W3 = range(7)
 PREFILL_FP32, PREFILL_MFMA, PREFILL_COLUMNS = 0, 1, 2
+F32, F16, BF16 = 0, 1, 2                             # rows and logits of the operators on device memory
+KV_TYPES = {"i8": 0, "e4m3": 1, "f16": 2, "bf16": 3}  # what a pool of pages holds
 
 
 class L2Error(RuntimeError):
@@ -38,6 +40,21 @@ class Config(C.Structure):
 
     def __repr__(self):
         return "Config { " + ", ".join(f"{n}: {getattr(self, n)}" for n, _ in self._fields_) + " }"
+
+
+class KvBatch(C.Structure):
+    """l2_kvbatch: the sequences of a call on a pool (device arrays as addresses, and their limits)."""
+    _fields_ = [("starts", C.c_void_p), ("lengths", C.c_void_p), ("pages", C.c_void_p)] + \
+        [(n, C.c_int32) for n in ("n_seqs", "max_pages", "n_rows", "max_rows", "max_length")]
+
+
+class Attention(C.Structure):
+    _fields_ = [("n_heads", C.c_int32), ("type", C.c_int32), ("scale", C.c_float), ("window", C.c_int32), ("sinks", C.c_int32),
+                ("q_stride", C.c_int64), ("out_stride", C.c_int64)]
+
+
+class Sampling(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("temperature", "top_k", "top_p", "min_p", "u")]
 
 
 # name: (restype, argtypes) — must list every symbol include/llama2_hip.h declares
@@ -86,6 +103,16 @@ SIGNATURES = {
     "l2_random_sample": (_I, [_VP, _VP, _I]),
     "l2_generate": (_I, [_VP, _VP, _VP, C.c_char_p, _I, _VP, C.c_float, _I, _VP, _SZ, C.POINTER(_I),
                          C.POINTER(C.c_int64)]),
+    "l2_kvpool_create": (_I, [_I, _I, _I, _I, _I, _I, C.POINTER(_VP)]),
+    "l2_kvpool_free": (None, [_VP]),
+    "l2_kvpool_bytes": (_SZ, [_VP]),
+    "l2_kvpool_write": (_I, [_VP, _I, C.POINTER(KvBatch), _VP, _VP, _I, C.c_int64, C.c_int64, _VP]),
+    "l2_kvpool_read": (_I, [_VP, _I, C.POINTER(KvBatch), _VP, _VP, _I, C.c_int64, C.c_int64, _VP]),
+    "l2_kvpool_attention_workspace": (_I, [_VP, C.POINTER(KvBatch), C.POINTER(Attention), C.POINTER(_SZ)]),
+    "l2_kvpool_attention": (_I, [_VP, _I, C.POINTER(KvBatch), C.POINTER(Attention), _VP, _VP, _VP, _SZ, _VP]),
+    "l2_sample_device": (_I, [_VP, _I, _I, _I, C.c_int64, C.POINTER(Sampling), _VP, _VP]),
+    "l2_decode_sample": (_I, [_VP, _VP, C.c_int32, C.c_int32, C.c_float, C.c_int32, C.c_float, C.c_float, C.c_float,
+                              C.POINTER(C.c_int32)]),
     "l2_qlinear_bench": (_I, [C.POINTER(_VP), _I, _I, C.POINTER(C.c_float)]),
     "l2_qlinear_bench_dispatch": (_I, [C.POINTER(_VP), _I, _I, C.POINTER(C.c_float)]),
     "l2_qlinear_kernel": (_I, [_VP, C.c_char_p, _SZ]),

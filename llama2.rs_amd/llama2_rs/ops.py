@@ -141,6 +141,74 @@ def qlinear_kernel(q) -> str:
     return buf.value.decode()
 
 
+def KvBatch(starts: int, lengths: int, pages: int, n_seqs: int, max_pages: int, n_rows: int, max_rows: int, max_length: int) -> _lib.KvBatch:
+    """The sequences of a call on a pool: device addresses of int32 arrays starts [n_seqs + 1], lengths [n_seqs] and pages
+    [n_seqs][max_pages], and the limits that hold for what they contain (l2_kvbatch)."""
+    return _lib.KvBatch(starts, lengths, pages, n_seqs, max_pages, n_rows, max_rows, max_length)
+
+
+class KvPool:
+    """Keys and values of many sequences in pages, in 8 or 16 bits ("i8", "e4m3", "f16", "bf16").  Rows, outputs and the
+    workspace are DEVICE addresses (integers) and work is enqueued on `stream` without waiting, as in QLinear.matvec_device;
+    `type` is _lib.F32, F16 or BF16, strides count elements from row to row (0: dense)."""
+
+    def __init__(self, n_layers: int, n_pages: int, page_size: int, n_kv_heads: int, head_size: int = 128, kv_type: str = "i8"):
+        if kv_type not in _lib.KV_TYPES:
+            raise ValueError(f"kv_type {kv_type!r} ({', '.join(_lib.KV_TYPES)})")
+        self.h = C.c_void_p()
+        check(lib().l2_kvpool_create(n_layers, n_pages, page_size, n_kv_heads, head_size, _lib.KV_TYPES[kv_type], C.byref(self.h)))
+
+    @property
+    def nbytes(self) -> int:
+        return lib().l2_kvpool_bytes(self.h)
+
+    def write(self, layer: int, batch, k: int, v: int, type: int = _lib.F32, k_stride: int = 0, v_stride: int = 0, stream: int = 0) -> None:
+        """Quantises the batch's rows into their slots."""
+        rc = lib().l2_kvpool_write(self.h, layer, batch, k, v, type, k_stride, v_stride, stream or None)
+        if rc:
+            check(rc)
+
+    def read(self, layer: int, batch, k: int, v: int, type: int = _lib.F32, k_stride: int = 0, v_stride: int = 0, stream: int = 0) -> None:
+        """What the pool holds at the batch's rows."""
+        rc = lib().l2_kvpool_read(self.h, layer, batch, k, v, type, k_stride, v_stride, stream or None)
+        if rc:
+            check(rc)
+
+    def attention_workspace(self, batch, n_heads: int, type: int = _lib.F32, window: int = 0, sinks: int = 0) -> int:
+        """Bytes of device memory that attention on such a batch wants as its workspace."""
+        n = C.c_size_t()
+        check(lib().l2_kvpool_attention_workspace(self.h, batch, _lib.Attention(n_heads, type, 0.0, window, sinks, 0, 0), C.byref(n)))
+        return n.value
+
+    def attention(self, layer: int, batch, q: int, out: int, n_heads: int, type: int = _lib.F32, scale: float = 0.0, window: int = 0,
+                  sinks: int = 0, workspace: int = 0, workspace_bytes: int = 0, q_stride: int = 0, out_stride: int = 0,
+                  stream: int = 0) -> None:
+        """Attention of the batch's rows over the pool (l2_kvpool_attention); scale 0: 1 / sqrt(head_size)."""
+        rc = lib().l2_kvpool_attention(self.h, layer, batch, _lib.Attention(n_heads, type, scale, window, sinks, q_stride, out_stride), q,
+                                       out, workspace or None, workspace_bytes, stream or None)
+        if rc:
+            check(rc)
+
+    def close(self):
+        if self.h:
+            lib().l2_kvpool_free(self.h)
+            self.h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def sample_device(logits: int, rows: int, vocab: int, ids: int, u: int, temperature: int = 0, top_k: int = 0, top_p: int = 0,
+                  min_p: int = 0, type: int = _lib.F32, stride: int = 0, stream: int = 0) -> None:
+    """One token id per row of logits (l2_sample_device); all addresses are DEVICE pointers, 0 leaves a setting off."""
+    rc = lib().l2_sample_device(logits, type, rows, vocab, stride, _lib.Sampling(temperature, top_k, top_p, min_p, u), ids, stream or None)
+    if rc:
+        check(rc)
+
+
 def copy_bench(nbytes: int, iters: int) -> float:
     ms = C.c_float()
     check(lib().l2_copy_bench(nbytes, iters, C.byref(ms)))
@@ -220,6 +288,13 @@ class Model:
     def decode_greedy(self, token: int, pos: int) -> int:
         nxt = C.c_int32()
         check(lib().l2_decode_greedy(self.h, self.state, token, pos, C.byref(nxt)))
+        return nxt.value
+
+    def decode_sample(self, token: int, pos: int, u: float, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                      min_p: float = 0.0) -> int:
+        """A step that samples from the logits on the device with the random number u in [0, 1) (l2_decode_sample)."""
+        nxt = C.c_int32()
+        check(lib().l2_decode_sample(self.h, self.state, token, pos, temperature, top_k, top_p, min_p, u, C.byref(nxt)))
         return nxt.value
 
     def generate_greedy(self, prompt_ids, steps: int, use_prefill: bool = True):
