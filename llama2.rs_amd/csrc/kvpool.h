@@ -37,6 +37,7 @@ struct KvAttention {
 // How the limits of a call are cut up: a function of them alone.
 struct KvAttnPlan {
     size_t workspace; // bytes
+    int splits;       // parts of the positions of short sequences
 };
 void kv_attention_plan(const KvLayer &l, int kv_type, const l2_kvbatch &b, const KvAttention &a, KvAttnPlan *plan);
 int kv_attention_launch(const KvLayer &l, int kv_type, const l2_kvbatch &b, const KvAttention &a, const KvAttnPlan &plan, void *workspace,
