@@ -103,6 +103,14 @@ __device__ __forceinline__ f8 load8(const void *p, int type, int64_t i) {
     return x;
 }
 
+__device__ __forceinline__ void store4(void *p, int type, int64_t i, const f4 &v) {
+    typedef _Float16 anyh __attribute__((ext_vector_type(4), aligned(2)));
+    typedef uint16_t anyb __attribute__((ext_vector_type(4), aligned(2)));
+    if (type == L2_F32) *(float4_any *)((float *)p + i) = float4_any{v[0], v[1], v[2], v[3]};
+    else if (type == L2_F16) *(anyh *)((_Float16 *)p + i) = anyh{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+    else *(anyb *)((uint16_t *)p + i) = anyb{kv::float_bf16(v[0]), kv::float_bf16(v[1]), kv::float_bf16(v[2]), kv::float_bf16(v[3])};
+}
+
 // The positions that the rows of a tile of queries have to do with, in tiles of TT: those of the first tokens that stay visible, then those from the
 // first row's window (or from the start) to the last row's own.
 struct Range {
@@ -135,7 +143,7 @@ struct Parts {
 // four waves tiles of 64 positions (32 of 16-bit cells) in turn, straight from memory into registers: 8 KB of keys and 8 KB of values, the next tile's keys
 // asked for once this one's scores are there and its values once this one's are summed.
 template <int KV, int NP, int D>
-__global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, int splits) {
+__global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, int splits, int stride) {
     using C = Cells<KV>;
     using Frag = typename C::Frag;
     constexpr int TT = 64 / C::kSize, ST = TT / 16, CH = TT / 4, FR = 2 / C::kSize, KL = D * C::kSize / 64, DT = D / 16, VS = TT / 32;
@@ -359,24 +367,28 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
         }
         const int64_t row = s.first + r / group, hq = h * group + r % group;
         if (splits == 1) {
-            for (int j = 0; j < 4; j++) kv::store(a.out, a.type, row * a.out_stride + hq * D + d + j, total == 0.f ? 0.f : v[j] / total);
+            const float inv = total == 0.f ? 0.f : 1.f / total;
+            for (int j = 0; j < 4; j++) v[j] = total == 0.f ? 0.f : v[j] * inv;
+            store4(a.out, a.type, row * a.out_stride + hq * D + d, v);
         } else {
-            const int64_t at = (row * a.n_heads + hq) * splits + split;
+            const int64_t at = (row * a.n_heads + hq) * stride + split;
             *(f4 *)(parts.acc + at * D + d) = v;
             if (d == 0) parts.stat[at] = make_float2(o, total);
         }
     }
 }
 
-// Joins the splits of each query row: one wave per row and head of a sequence that the kernel above takes.
+// Joins the splits of each query row: one wave per row and head.
 template <int D>
-__global__ __launch_bounds__(64) void kv_join_kernel(l2_kvbatch b, KvAttention a, Parts parts, int splits, int group) {
+__global__ __launch_bounds__(64) void kv_join_kernel(l2_kvbatch b, KvAttention a, Parts parts, int narrow, int wide, int stride, int group) {
     const int row = blockIdx.x, hq = blockIdx.y, lane = threadIdx.x;
     const int i = kv::sequence_of(b, row);
     if (i >= b.n_seqs) return;
     const kv::Seq s = kv::sequence(b, i);
-    if (row - s.first >= s.rows || s.rows * group > kNarrowRows) return;
-    const int64_t at = ((int64_t)row * a.n_heads + hq) * splits;
+    if (row - s.first >= s.rows) return;
+    const int splits = (int64_t)s.rows * group > kNarrowRows ? wide : narrow;
+    if (splits == 1) return;
+    const int64_t at = ((int64_t)row * a.n_heads + hq) * stride;
     float o = -kInf, total = 0.f;
     for (int x = 0; x < splits; x++) o = fmaxf(o, parts.stat[at + x].x);
     constexpr int E = D / 64;
@@ -391,67 +403,314 @@ __global__ __launch_bounds__(64) void kv_join_kernel(l2_kvbatch b, KvAttention a
     for (int e = 0; e < E; e++) kv::store(a.out, a.type, row * a.out_stride + (int64_t)hq * D + E * lane + e, total == 0.f ? 0.f : v[e] / total);
 }
 
-// One block per row and query head; its four waves take positions in turn, each with a running maximum and sum, and are joined at the end.
-template <int KV, int D>
-__global__ __launch_bounds__(256) void kv_attention_kernel(KvLayer l, l2_kvbatch b, KvAttention a) {
-    const int row = blockIdx.x, hq = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int i = kv::sequence_of(b, row);
-    if (i >= b.n_seqs) return;
-    const kv::Seq s = kv::sequence(b, i);
-    const int at = row - s.first, pos = s.length - s.rows + at;
-    if (at >= s.rows || s.rows * (a.n_heads / l.n_heads) <= kNarrowRows) return;
-    const int h = hq / (a.n_heads / l.n_heads);
-    constexpr int E = D / 64;
-    float q[E], acc[E] = {}, m = -__builtin_inff(), sum = 0.f;
-    for (int e = 0; e < E; e++) q[e] = kv::load(a.q, a.type, row * a.q_stride + (int64_t)hq * D + 64 * e + lane);
-    const int size = 1 << l.page_shift;
-    for (int t = w; t <= pos; t += 4) {
-        if (a.window && t <= pos - a.window && t >= a.sinks) continue;
-        const int page = kv::page_at(b, l.n_pages, i, t >> l.page_shift);
-        if (page < 0) continue;
-        const int slot = t & (size - 1);
-        const int64_t ph = (int64_t)page * l.n_heads + h;
-        float kx[E], vx[E], dot = 0.f;
-        const float ks = KV <= L2_KV_E4M3 ? l.k_scale[ph * size + slot] : 1.f, vs = KV <= L2_KV_E4M3 ? l.v_scale[ph * size + slot] : 1.f;
-        for (int e = 0; e < E; e++) {
-            const int64_t ki = (ph * size + slot) * D + 64 * e + lane, vi = (ph * D + 64 * e + lane) * size + slot;
-            if (KV == L2_KV_I8) kx[e] = (float)((const int8_t *)l.k)[ki], vx[e] = (float)((const int8_t *)l.v)[vi];
-            else if (KV == L2_KV_E4M3) kx[e] = kv::from_e4m3(((const uint8_t *)l.k)[ki]), vx[e] = kv::from_e4m3(((const uint8_t *)l.v)[vi]);
-            else if (KV == L2_KV_F16) kx[e] = (float)((const _Float16 *)l.k)[ki], vx[e] = (float)((const _Float16 *)l.v)[vi];
-            else kx[e] = kv::bf16_float(((const uint16_t *)l.k)[ki]), vx[e] = kv::bf16_float(((const uint16_t *)l.v)[vi]);
-            dot += q[e] * kx[e];
-        }
-        for (int o = 32; o; o >>= 1) dot += __shfl_xor(dot, o);
-        dot *= ks * a.scale;
-        const float mm = dot > m || dot != dot ? dot : m, f = m == mm ? 1.f : expf(m - mm), p = dot == mm ? 1.f : expf(dot - mm);
-        sum = sum * f + p;
-        for (int e = 0; e < E; e++) acc[e] = acc[e] * f + p * (vx[e] * vs);
-        m = mm;
-    }
-    __shared__ float sm[4], ss[4], sa[4][D];
-    if (lane == 0) sm[w] = m, ss[w] = sum;
-    for (int e = 0; e < E; e++) sa[w][64 * e + lane] = acc[e];
-    __syncthreads();
-    if (w) return;
-    float top = -__builtin_inff(), total = 0.f;
-    for (int x = 0; x < 4; x++) top = sm[x] > top || sm[x] != sm[x] ? sm[x] : top;
-    float o[E] = {};
-    for (int x = 0; x < 4; x++) {
-        if (ss[x] == 0.f) continue;
-        const float f = sm[x] == top ? 1.f : expf(sm[x] - top);
-        total += ss[x] * f;
-        for (int e = 0; e < E; e++) o[e] += sa[x][64 * e + lane] * f;
-    }
-    for (int e = 0; e < E; e++) kv::store(a.out, a.type, row * a.out_stride + (int64_t)hq * D + 64 * e + lane, total == 0.f ? 0.f : o[e] / total);
+typedef float f16v __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ f16v mfma32(const h8 &a, const h8 &b, const f16v &c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f16v mfma32(const b8 &a, const b8 &b, const f16v &c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+
+constexpr int kWideWaves = 4, kWideRows = 32 * kWideWaves, kWideThreads = 64 * kWideWaves;
+
+// Where 16-byte piece x of row r lies in a tile of rows of 128 (256) bytes: the sixteen rows that a 16-byte LDS read takes together then meet sixteen places.
+template <int PER_ROW>
+__device__ __forceinline__ int piece_at(int r, int x) {
+    return r * PER_ROW + (PER_ROW == 16 ? x ^ (r & 15) : x ^ (r >> 1 & 7));
 }
 
-typedef void (*AttnKernel)(KvLayer, l2_kvbatch, KvAttention);
-const AttnKernel kAttn[4][2] = {{kv_attention_kernel<0, 64>, kv_attention_kernel<0, 128>}, {kv_attention_kernel<1, 64>, kv_attention_kernel<1, 128>},
-                                {kv_attention_kernel<2, 64>, kv_attention_kernel<2, 128>}, {kv_attention_kernel<3, 64>, kv_attention_kernel<3, 128>}};
-typedef void (*NarrowKernel)(KvLayer, l2_kvbatch, KvAttention, Parts, int);
-#define NARROW(kv, np) {kv_narrow_kernel<kv, np, 64>, kv_narrow_kernel<kv, np, 128>}
-const NarrowKernel kNarrow[4][3][2] = {{NARROW(0, 1), NARROW(0, 2), {}}, {NARROW(1, 1), NARROW(1, 2), {}}, {NARROW(2, 1), NARROW(2, 2), {}}, {NARROW(3, 1), NARROW(3, 2), NARROW(3, 3)}};
-typedef void (*JoinKernel)(l2_kvbatch, KvAttention, Parts, int, int);
+// Longer chunks.  A block has 128 query rows of one sequence and kv head, a wave 32 of them; keys and values come in tiles of 64 positions through LDS,
+// in 16 bits, the next tile's bytes on their way into registers meanwhile.
+template <int KV, int NP, int D>
+__global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, int splits, int stride) {
+    using C = Cells<KV>;
+    using Frag = typename C::Frag;
+    constexpr int TT = 64, PK = D / 8, DT = D / 32, KS = D / 16, LOADS = TT * D * C::kSize / 16 / kWideThreads;
+    constexpr int ROW16 = D * C::kSize / 16;      // 16-byte pieces of a row of K in memory
+    constexpr int COL16 = TT * C::kSize / 16;     // and of the tile's part of a row of V
+    __shared__ __align__(16) u4 sh_k[2][TT * PK], sh_v[2][D * 8];
+    __shared__ __align__(16) float sh_ks[2][TT], sh_vs[2][TT];
+    __shared__ int sh_page[2][4], sh_odd[2], sh_seq, sh_tile;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, n = lane & 31, hh = lane >> 5;
+    const int group = a.n_heads / l.n_heads;
+    const int h = blockIdx.x % l.n_heads, split = blockIdx.x / l.n_heads % splits;
+
+    // which sequence's rows: the tiles of all sequences one behind the other
+    {
+        int at = blockIdx.x / (l.n_heads * splits);
+        if (tid == 0) sh_seq = -1;
+        if (tid < 2) sh_odd[tid] = -1;
+        __syncthreads();
+        for (int i0 = 0; i0 < b.n_seqs; i0 += 64) {
+            int tiles = 0;
+            if (i0 + lane < b.n_seqs) {
+                const int64_t r = (int64_t)kv::sequence(b, i0 + lane).rows * group;
+                tiles = r > kNarrowRows ? (int)((r + kWideRows - 1) / kWideRows) : 0;
+            }
+            int upto = tiles;
+            for (int o = 1; o < 64; o <<= 1) {
+                const int x = __shfl_up(upto, o);
+                if (lane >= o) upto += x;
+            }
+            if (w == 0 && upto > at && upto - tiles <= at) sh_seq = i0 + lane, sh_tile = tiles - 1 - (at - (upto - tiles)); // the longest first
+            const int all = __shfl(upto, 63);
+            if (at < all) break;
+            at -= all;
+        }
+        __syncthreads();
+    }
+    const int i = sh_seq;
+    if (i < 0) return;
+    const kv::Seq s = kv::sequence(b, i);
+    const int rows = s.rows * group, row0 = sh_tile * kWideRows + 32 * w, base = s.length - s.rows;
+    const bool real = row0 + n < rows;
+    const int tok = real ? (row0 + n) / group : 0;
+    const int pos = real ? base + tok : -1;
+    const int64_t q_row = s.first + tok, head = h * group + (real ? (row0 + n) % group : 0);
+    // the positions of the wave's rows and of the block's
+    const int w_first = base + min(row0, rows - 1) / group, w_last = row0 < rows ? base + (min(row0 + 32, rows) - 1) / group : -1;
+    const int b_first = base + sh_tile * kWideRows / group, b_last = base + (min((sh_tile + 1) * kWideRows, rows) - 1) / group;
+
+    Frag q[KS][NP];
+    float c;
+    {
+        float top = 0.f;
+        c = a.scale * kLog2e;
+        int e = 0;
+        if (C::kHalf) {
+            for (int k = 0; k < KS; k++) {
+                const f8 x = load8(a.q, a.type, q_row * a.q_stride + head * D + 16 * k + 8 * hh);
+                for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[j]));
+            }
+            const lanes::Both t = lanes::both32(top);
+            top = fmaxf(t.lo, t.hi);
+            e = top > 0.f && top < kInf ? 15 - __builtin_amdgcn_frexp_expf(top) : 0; // the largest in [2^14, 2^15)
+            c = ldexpf(c, -e);
+        }
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            f8 x = load8(a.q, a.type, q_row * a.q_stride + head * D + 16 * k + 8 * hh);
+            if (C::kHalf)
+                for (int j = 0; j < 8; j++) x[j] = ldexpf(x[j], e);
+            pieces<Frag, typename C::One, NP>(x, q[k]);
+        }
+    }
+
+    const Range range = range_of<TT>(a, b_first, b_last);
+    const int per = (range.n + splits - 1) / splits, begin = min(split * per, range.n), end = min(begin + per, range.n);
+    const int size = 1 << l.page_shift;
+
+    u4 kr[LOADS], vr[LOADS];
+    int pk[LOADS], pv[LOADS], page4 = -1; // pages of the tile that is asked for next
+    float scale = 0.f;
+    auto pages = [&](int x) {
+        const int t0 = range.tile(x) * TT;
+#pragma unroll
+        for (int y = 0; y < LOADS; y++) {
+            const int p = tid + kWideThreads * y;
+            pk[y] = kv::page_at(b, l.n_pages, i, (t0 + p / ROW16) >> l.page_shift);
+            pv[y] = kv::page_at(b, l.n_pages, i, (t0 + (p % COL16) * (16 / C::kSize)) >> l.page_shift);
+        }
+        // lanes 0..63 of waves 0 and 1: the scales' pages; threads 128..131: of the four quarters
+        const int t = t0 + (tid < 128 ? tid & 63 : 16 * (tid & 3));
+        if (C::kEight || tid >= 128) page4 = kv::page_at(b, l.n_pages, i, t >> l.page_shift);
+    };
+    auto load = [&](int x) {
+        const int t0 = range.tile(x) * TT;
+#pragma unroll
+        for (int y = 0; y < LOADS; y++) {
+            const int p = tid + kWideThreads * y, t = t0 + p / ROW16;
+            const int64_t ph = (int64_t)max(pk[y], 0) * l.n_heads + h;
+            kr[y] = *(const u4 *)((const char *)l.k + ((ph * size + (t & (size - 1))) * D * C::kSize + 16 * (p % ROW16)));
+        }
+#pragma unroll
+        for (int y = 0; y < LOADS; y++) {
+            const int p = tid + kWideThreads * y, t = t0 + (p % COL16) * (16 / C::kSize);
+            const int64_t ph = (int64_t)max(pv[y], 0) * l.n_heads + h;
+            vr[y] = *(const u4 *)((const char *)l.v + ((ph * D + p / COL16) * size + (t & (size - 1))) * C::kSize);
+        }
+        if (C::kEight && tid < 128)
+            scale = (tid < 64 ? l.k_scale : l.v_scale)[((int64_t)max(page4, 0) * l.n_heads + h) * size + ((t0 + (tid & 63)) & (size - 1))];
+    };
+    // Whether every row of first..last sees all of a tile whose pages are there.
+    auto all_visible = [&](int t0, int first, int last) { return t0 + TT - 1 <= first && (!a.window || t0 > last - a.window || t0 + TT <= a.sinks); };
+    auto stage = [&](int x, int buf) {
+        bool odd = false;
+        if (!C::kEight && !all_visible(range.tile(x) * TT, b_first, b_last)) { // values that are not finite are added one by one (below)
+            constexpr uint32_t ones = KV == L2_KV_F16 ? 0x7C00u : 0x7F80u;
+#pragma unroll
+            for (int y = 0; y < LOADS; y++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const uint32_t v = vr[y][r];
+                    const bool lo = (v & ones) == ones, hi = (v >> 16 & ones) == ones;
+                    odd |= lo || hi;
+                    vr[y][r] = v & ((lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u));
+                }
+        }
+#pragma unroll
+        for (int y = 0; y < LOADS; y++) {
+            const int p = tid + kWideThreads * y, kr_row = p / ROW16, kr_x = p % ROW16, v_row = p / COL16, v_x = p % COL16;
+            if constexpr (C::kEight) {
+                sh_k[buf][piece_at<PK>(kr_row, 2 * kr_x)] = __builtin_bit_cast(u4, C::frag(kr[y], 0));
+                sh_k[buf][piece_at<PK>(kr_row, 2 * kr_x + 1)] = __builtin_bit_cast(u4, C::frag(kr[y], 1));
+                sh_v[buf][piece_at<8>(v_row, 2 * v_x)] = __builtin_bit_cast(u4, C::frag(vr[y], 0));
+                sh_v[buf][piece_at<8>(v_row, 2 * v_x + 1)] = __builtin_bit_cast(u4, C::frag(vr[y], 1));
+            } else {
+                // a page that is not there lies over page 0: whatever that holds is hidden, but must be finite
+                sh_k[buf][piece_at<PK>(kr_row, kr_x)] = kr[y];
+                sh_v[buf][piece_at<8>(v_row, v_x)] = pv[y] < 0 ? u4{0, 0, 0, 0} : vr[y];
+            }
+        }
+        if (C::kEight && tid < 128) (tid < 64 ? sh_ks : sh_vs)[buf][tid & 63] = scale;
+        if (tid >= 128 && tid < 132) sh_page[buf][tid & 3] = page4;
+        if (odd) sh_odd[buf] = x;
+    };
+
+    f16v acc[DT] = {};
+    float top = -kInf, e = kLeastE, off = -kInf, sum = 0.f;
+    if (begin < end) {
+        pages(begin);
+        load(begin);
+        stage(begin, 0);
+        __syncthreads();
+    }
+    for (int x = begin; x < end; x++) {
+        const int buf = (x - begin) & 1, t0 = range.tile(x) * TT;
+        const bool more = x + 1 < end;
+        if (more) {
+            pages(x + 1);
+            load(x + 1);
+        }
+        const bool none = w_last < t0 || (a.window && t0 + TT - 1 <= w_first - a.window && t0 >= a.sinks);
+        if (!none) {
+            // scores of 2 x 32 positions: position 32 y + 16 s + 8 hh + 4 (b & 1) + r in element 4 b + r, b = 2 s + (b & 1)
+            f16v sc[2] = {};
+            const int kr_row = (n & 0x13) | (n & 4) << 1 | (n & 8) >> 1;
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+                    const Frag f = __builtin_bit_cast(Frag, sh_k[buf][piece_at<PK>(32 * y + kr_row, 2 * k + hh)]);
+#pragma unroll
+                    for (int z = 0; z < NP; z++) sc[y] = mfma32(f, q[k][z], sc[y]);
+                }
+            const bool there = sh_page[buf][0] >= 0 && sh_page[buf][1] >= 0 && sh_page[buf][2] >= 0 && sh_page[buf][3] >= 0;
+            const bool whole = there && all_visible(t0, w_first, w_last);
+            f4 vs[8];
+            if (C::kEight) {
+#pragma unroll
+                for (int z = 0; z < 8; z++) {
+                    const int t = 32 * (z / 4) + 16 * (z / 2 & 1) + 8 * hh + 4 * (z & 1);
+                    const f4 ks = *(const f4 *)&sh_ks[buf][t];
+                    vs[z] = *(const f4 *)&sh_vs[buf][t];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) sc[z / 4][4 * (z & 3) + r] *= ks[r];
+                }
+            }
+            if (!whole) {
+#pragma unroll
+                for (int z = 0; z < 8; z++) {
+                    const int t = 32 * (z / 4) + 16 * (z / 2 & 1) + 8 * hh + 4 * (z & 1);
+                    const bool here = sh_page[buf][t >> 4] >= 0;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const bool see = here && visible(a, t0 + t + r, pos);
+                        sc[z / 4][4 * (z & 3) + r] = see ? sc[z / 4][4 * (z & 3) + r] : -kInf;
+                        if (C::kEight) vs[z][r] = see ? vs[z][r] : 0.f;
+                    }
+                }
+            }
+            float mx = -kInf, mv = 0.f;
+#pragma unroll
+            for (int z = 0; z < 8; z++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    mx = fmaxf(mx, sc[z / 4][4 * (z & 3) + r]);
+                    if (C::kEight) mv = fmaxf(mv, vs[z][r]);
+                }
+            const lanes::Both m2 = lanes::both32(mx);
+            top = fmaxf(top, fmaxf(m2.lo, m2.hi) * c);
+            if (C::kEight) {
+                const lanes::Both v2 = lanes::both32(mv);
+                mv = fmaxf(v2.lo, v2.hi);
+                if (mv > 0.f) e = fmaxf(e, (float)__builtin_amdgcn_frexp_expf(mv));
+            }
+            const float now = top == -kInf ? 0.f : C::kEight ? top + (e - 15.f) : C::kHalf ? top - 15.f : top;
+            const float f = off == now ? 1.f : __builtin_amdgcn_exp2f(off - now);
+            if (__ballot(f != 1.f)) {
+#pragma unroll
+                for (int y = 0; y < DT; y++) acc[y] *= f;
+                sum *= f;
+            }
+            off = top == -kInf ? -kInf : now;
+#pragma unroll
+            for (int v = 0; v < 4; v++) { // positions 16 v + 8 hh + j
+                f8 p;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int z = 2 * v + j / 4;
+                    const float t = __builtin_amdgcn_exp2f(fmaf(sc[z / 4][4 * (z & 3) + j % 4], c, -now));
+                    sum += t;
+                    p[j] = C::kEight ? t * vs[z][j % 4] : t;
+                }
+                Frag pf[NP];
+                pieces<Frag, typename C::One, NP>(p, pf);
+#pragma unroll
+                for (int y = 0; y < DT; y++) {
+                    const Frag fr = __builtin_bit_cast(Frag, sh_v[buf][piece_at<8>(32 * y + n, 2 * v + hh)]);
+#pragma unroll
+                    for (int z = 0; z < NP; z++) acc[y] = mfma32(fr, pf[z], acc[y]);
+                }
+            }
+            if (!C::kEight && sh_odd[buf] == x) {
+                for (int y = 0; y < TT; y++) {
+                    const int t = t0 + y, page = kv::page_at(b, l.n_pages, i, t >> l.page_shift);
+                    if (page < 0 || !visible(a, t, pos)) continue;
+                    const uint16_t *p = (const uint16_t *)l.v + (((int64_t)page * l.n_heads + h) * D * size + (t & (size - 1)));
+#pragma unroll
+                    for (int z = 0; z < DT; z++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) {
+                            const uint16_t bits = p[(int64_t)(32 * z + 8 * (r / 4) + 4 * hh + r % 4) * size];
+                            const float v = KV == L2_KV_F16 ? (float)__builtin_bit_cast(_Float16, bits) : kv::bf16_float(bits);
+                            if (!(fabsf(v) < kInf)) acc[z][r] += v;
+                        }
+                }
+            }
+        }
+        if (more) stage(x + 1, buf ^ 1);
+        __syncthreads();
+    }
+    const lanes::Both s2 = lanes::both32(sum);
+    sum = s2.lo + s2.hi;
+    if (!real) return;
+    if (splits == 1) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int y = 0; y < DT; y++)
+#pragma unroll
+            for (int z = 0; z < 4; z++) {
+                const int64_t at = q_row * a.out_stride + head * D + 32 * y + 8 * z + 4 * hh;
+                f4 v;
+#pragma unroll
+                for (int r = 0; r < 4; r++) v[r] = sum == 0.f ? 0.f : acc[y][4 * z + r] * inv;
+                store4(a.out, a.type, at, v);
+            }
+    } else {
+        const int64_t at = (q_row * a.n_heads + head) * stride + split;
+#pragma unroll
+        for (int y = 0; y < DT; y++)
+#pragma unroll
+            for (int z = 0; z < 4; z++)
+                *(f4 *)(parts.acc + at * D + 32 * y + 8 * z + 4 * hh) = f4{acc[y][4 * z], acc[y][4 * z + 1], acc[y][4 * z + 2], acc[y][4 * z + 3]};
+        if (hh == 0) parts.stat[at] = make_float2(off, sum);
+    }
+}
+
+typedef void (*AttnKernel)(KvLayer, l2_kvbatch, KvAttention, Parts, int, int);
+#define SIZES(kernel, kv, np) {kernel<kv, np, 64>, kernel<kv, np, 128>}
+#define ALL(kernel)                                                                                                                             \
+    {{SIZES(kernel, 0, 1), SIZES(kernel, 0, 2), {}}, {SIZES(kernel, 1, 1), SIZES(kernel, 1, 2), {}}, {SIZES(kernel, 2, 1), SIZES(kernel, 2, 2), {}}, \
+     {SIZES(kernel, 3, 1), SIZES(kernel, 3, 2), SIZES(kernel, 3, 3)}}
+const AttnKernel kNarrow[4][3][2] = ALL(kv_narrow_kernel), kWide[4][3][2] = ALL(kv_wide_kernel);
+typedef void (*JoinKernel)(l2_kvbatch, KvAttention, Parts, int, int, int, int);
 const JoinKernel kJoin[2] = {kv_join_kernel<64>, kv_join_kernel<128>};
 
 // In how many 16-bit numbers q and the weights enter the matrix cores, less one.
@@ -463,36 +722,54 @@ int pieces_index(int kv_type, int type) {
 } // namespace
 
 void kv_attention_plan(const KvLayer &l, int kv_type, const l2_kvbatch &b, const KvAttention &a, KvAttnPlan *plan) {
-    const int tt = kv_type <= L2_KV_E4M3 ? 64 : 32;
-    int64_t seen = b.max_length; // positions of the longest row
-    if (a.window) seen = std::min<int64_t>(seen, (int64_t)a.window + b.max_rows + a.sinks + 2 * tt);
-    const int64_t tiles = (seen + tt - 1) / tt, blocks = (int64_t)std::max(b.n_seqs, 1) * l.n_heads;
-    const int64_t want = (2 * cu_count() + blocks - 1) / blocks;
-    plan->splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, tiles / (2 * kNarrowWaves)));
-    const size_t cells = (size_t)b.n_rows * a.n_heads * plan->splits;
-    plan->workspace = plan->splits > 1 ? cells * (l.head_size * 4 + 8) : 0;
+    const int group = a.n_heads / l.n_heads;
+    const int64_t rows = std::min(b.max_rows, b.n_rows), seqs = std::max(b.n_seqs, 1);
+    auto tiles_seen = [&](int64_t tt, int64_t per_tile) { // of the row tile that sees most
+        int64_t seen = b.max_length;
+        if (a.window) seen = std::min<int64_t>(seen, (int64_t)a.window + std::min(rows, per_tile) + a.sinks + 2 * tt);
+        return (seen + tt - 1) / tt;
+    };
+    auto parts_of = [&](int64_t blocks, int64_t full, int64_t tiles, int64_t least) {
+        return (int)std::max<int64_t>(1, std::min<int64_t>((full + blocks - 1) / blocks, tiles / least));
+    };
+    plan->narrow = group <= kNarrowRows;
+    plan->wide = rows * group > kNarrowRows;
+    plan->narrow_splits = plan->wide_splits = 1;
+    if (plan->narrow)
+        plan->narrow_splits = parts_of(seqs * l.n_heads, 2 * cu_count(), tiles_seen(kv_type <= L2_KV_E4M3 ? 64 : 32, kNarrowRows), 2 * kNarrowWaves);
+    // row tiles of all sequences, at most: their whole ones, and a last one of each that has more rows than the narrow kernel takes
+    const int64_t all = (int64_t)b.n_rows * group;
+    plan->wide_tiles = (int)std::min<int64_t>(all / kWideRows + std::min<int64_t>(seqs, all / (kNarrowRows + 1)), 1 << 26);
+    if (plan->wide) plan->wide_splits = parts_of(std::max<int64_t>(plan->wide_tiles, 1) * l.n_heads, cu_count(), tiles_seen(64, (kWideRows + group - 1) / group), 4);
+    plan->stride = std::max(plan->narrow_splits, plan->wide_splits);
+    plan->workspace = plan->stride > 1 ? (size_t)b.n_rows * a.n_heads * plan->stride * (l.head_size * 4 + 8) : 0;
 }
 
 int kv_attention_launch(const KvLayer &l, int kv_type, const l2_kvbatch &b, const KvAttention &a, const KvAttnPlan &plan, void *workspace, hipStream_t st) {
     if (b.n_rows == 0 || b.n_seqs == 0 || b.max_rows == 0) return L2_OK;
-    const int wide = l.head_size == 128, group = a.n_heads / l.n_heads;
+    const int big = l.head_size == 128, group = a.n_heads / l.n_heads, np = pieces_index(kv_type, a.type);
     Parts parts{(float *)workspace, nullptr};
-    parts.stat = (float2 *)(parts.acc + (size_t)b.n_rows * a.n_heads * plan.splits * l.head_size);
-    if (group <= kNarrowRows) {
-        l2_launch(kNarrow[kv_type][pieces_index(kv_type, a.type)][wide], dim3(plan.splits, l.n_heads, b.n_seqs), dim3(64 * kNarrowWaves), 0, st, l, b, a, parts,
-                  plan.splits);
-        if (plan.splits > 1) l2_launch(kJoin[wide], dim3(b.n_rows, a.n_heads), dim3(64), 0, st, b, a, parts, plan.splits, group);
+    parts.stat = (float2 *)(parts.acc + (size_t)b.n_rows * a.n_heads * plan.stride * l.head_size);
+    if (plan.wide && plan.wide_tiles) {
+        const int64_t blocks = (int64_t)plan.wide_tiles * l.n_heads * plan.wide_splits;
+        if (blocks >= (int64_t)1 << 31) return l2_fail(L2_ERR_RANGE, "%d rows of %d heads", b.n_rows, a.n_heads);
+        l2_launch(kWide[kv_type][np][big], dim3((unsigned)blocks), dim3(kWideThreads), 0, st, l, b, a, parts, plan.wide_splits, plan.stride);
     }
-    if ((int64_t)b.max_rows * group > kNarrowRows)
-        l2_launch(kAttn[kv_type][wide], dim3(b.n_rows, a.n_heads), dim3(256), 0, st, l, b, a);
+    if (plan.narrow)
+        l2_launch(kNarrow[kv_type][np][big], dim3(plan.narrow_splits, l.n_heads, b.n_seqs), dim3(64 * kNarrowWaves), 0, st, l, b, a, parts, plan.narrow_splits,
+                  plan.stride);
+    if (plan.stride > 1) l2_launch(kJoin[big], dim3(b.n_rows, a.n_heads), dim3(64), 0, st, b, a, parts, plan.narrow_splits, plan.wide_splits, plan.stride, group);
     L2_HIP(hipGetLastError());
     return L2_OK;
 }
 
 int kv_attention_warm_up() {
     hipFuncAttributes a;
-    for (auto &k : kAttn) for (AttnKernel f : k) L2_HIP(hipFuncGetAttributes(&a, (const void *)f));
-    for (auto &k : kNarrow) for (auto &n : k) for (NarrowKernel f : n) if (f) L2_HIP(hipFuncGetAttributes(&a, (const void *)f));
+    for (auto &all : {&kNarrow, &kWide})
+        for (auto &k : *all)
+            for (auto &n : k)
+                for (AttnKernel f : n)
+                    if (f) L2_HIP(hipFuncGetAttributes(&a, (const void *)f));
     for (JoinKernel f : kJoin) L2_HIP(hipFuncGetAttributes(&a, (const void *)f));
     return L2_OK;
 }

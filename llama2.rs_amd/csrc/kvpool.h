@@ -36,8 +36,11 @@ struct KvAttention {
 };
 // How the limits of a call are cut up: a function of them alone.
 struct KvAttnPlan {
-    size_t workspace; // bytes
-    int splits;       // parts of the positions of short sequences
+    size_t workspace;               // bytes
+    bool narrow, wide;              // which kernels there may be sequences for
+    int narrow_splits, wide_splits; // parts that positions are cut into
+    int stride;                     // the larger of both: parts of a row in the workspace
+    int wide_tiles;                 // tiles of rows of the wide kernel, at most
 };
 void kv_attention_plan(const KvLayer &l, int kv_type, const l2_kvbatch &b, const KvAttention &a, KvAttnPlan *plan);
 int kv_attention_launch(const KvLayer &l, int kv_type, const l2_kvbatch &b, const KvAttention &a, const KvAttnPlan &plan, void *workspace,
