@@ -131,6 +131,19 @@ __device__ __forceinline__ bool visible(const KvAttention &a, int t, int pos) {
     return t <= pos && (!a.window || t > pos - a.window || t < a.sinks);
 }
 
+// v with fp16 (bf16) numbers that are not finite as zeros, and whether there are any.
+template <int KV>
+__device__ __forceinline__ u4 finite(u4 v, bool &odd) {
+    constexpr uint32_t ones = KV == L2_KV_F16 ? 0x7C00u : 0x7F80u;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const bool lo = (v[r] & ones) == ones, hi = (v[r] >> 16 & ones) == ones;
+        odd |= lo || hi;
+        v[r] &= (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u);
+    }
+    return v;
+}
+
 constexpr int kNarrowRows = 16, kNarrowWaves = 4;
 
 // A query row's part: what a block found of it.  `off` is common to the weights in acc and sum.
@@ -265,18 +278,9 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
                     sc[x][r] = see ? sc[x][r] : -kInf;
                     if (C::kEight) vs[x][r] = see ? vs[x][r] : 0.f;
                 }
-            if (!C::kEight) {
-                constexpr uint32_t ones = KV == L2_KV_F16 ? 0x7C00u : 0x7F80u;
+            if (!C::kEight)
 #pragma unroll
-                for (int x = 0; x < DT; x++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const uint32_t v = vr[x][r];
-                        const bool lo = (v & ones) == ones, hi = (v >> 16 & ones) == ones;
-                        odd |= lo || hi;
-                        vr[x][r] = v & ((lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u));
-                    }
-            }
+                for (int x = 0; x < DT; x++) vr[x] = finite<KV>(vr[x], odd);
         }
         float mx = -kInf;
 #pragma unroll
@@ -415,19 +419,39 @@ __device__ __forceinline__ int piece_at(int r, int x) {
     return r * PER_ROW + (PER_ROW == 16 ? x ^ (r & 15) : x ^ (r >> 1 & 7));
 }
 
-// Longer chunks.  A block has 128 query rows of one sequence and kv head, a wave 32 of them; keys and values come in tiles of 64 positions through LDS,
-// in 16 bits, the next tile's bytes on their way into registers meanwhile.
+// Values that are the same in every lane, in scalar registers.
+__device__ __forceinline__ kv::Seq uniform(const kv::Seq &s) {
+    return {__builtin_amdgcn_readfirstlane(s.first), __builtin_amdgcn_readfirstlane(s.rows), __builtin_amdgcn_readfirstlane(s.length)};
+}
+// A word of memory that nothing writes while the kernel runs, at an address that is the same in every lane.
+__device__ __forceinline__ int uniform_load(const int32_t *p) { return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)p; }
+
+// From memory (a base that is the same in every lane, and an offset of each, or each lane's address) into LDS, lane l's 16 bytes to `lds` + 16 l.  The compiler
+// does not know of these loads: wait_lds_loads() before the barrier behind which they are read.
+__device__ __forceinline__ void lds_load(uint32_t lds, const char *base, uint32_t off) {
+    const uint64_t p = (uint64_t)base;
+    const uint64_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)p) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(at) : "memory", "m0");
+}
+__device__ __forceinline__ void lds_load(uint32_t lds, const char *at) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(at) : "memory", "m0");
+}
+__device__ __forceinline__ void wait_lds_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Longer chunks.  A block has 128 query rows of one sequence and kv head, a wave 32 of them; keys and values come in tiles of 64 positions through LDS, in 16
+// bits, the next tile on its way meanwhile: codes of 8 bits into registers, to be converted once for all four waves, 16-bit cells straight into LDS.  A tile is
+// four runs of 16 positions, each in one page; their addresses are computed once per wave.
 template <int KV, int NP, int D>
 __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, int splits, int stride) {
     using C = Cells<KV>;
     using Frag = typename C::Frag;
     constexpr int TT = 64, PK = D / 8, DT = D / 32, KS = D / 16, LOADS = TT * D * C::kSize / 16 / kWideThreads;
-    constexpr int ROW16 = D * C::kSize / 16;      // 16-byte pieces of a row of K in memory
-    constexpr int COL16 = TT * C::kSize / 16;     // and of the tile's part of a row of V
+    constexpr int RUN = 16 * D * C::kSize;        // bytes of 16 rows of K
+    constexpr int COL16 = TT * C::kSize / 16;     // 16-byte pieces of the tile's part of a row of V
     __shared__ __align__(16) u4 sh_k[2][TT * PK], sh_v[2][D * 8];
     __shared__ __align__(16) float sh_ks[2][TT], sh_vs[2][TT];
-    __shared__ int sh_page[2][4], sh_odd[2], sh_seq, sh_tile;
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, n = lane & 31, hh = lane >> 5;
+    __shared__ int sh_seq, sh_tile;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, hh = lane >> 5;
     const int group = a.n_heads / l.n_heads;
     const int h = blockIdx.x % l.n_heads, split = blockIdx.x / l.n_heads % splits;
 
@@ -435,7 +459,6 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
     {
         int at = blockIdx.x / (l.n_heads * splits);
         if (tid == 0) sh_seq = -1;
-        if (tid < 2) sh_odd[tid] = -1;
         __syncthreads();
         for (int i0 = 0; i0 < b.n_seqs; i0 += 64) {
             int tiles = 0;
@@ -455,17 +478,17 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
         }
         __syncthreads();
     }
-    const int i = sh_seq;
+    const int i = __builtin_amdgcn_readfirstlane(sh_seq), tile = __builtin_amdgcn_readfirstlane(sh_tile);
     if (i < 0) return;
-    const kv::Seq s = kv::sequence(b, i);
-    const int rows = s.rows * group, row0 = sh_tile * kWideRows + 32 * w, base = s.length - s.rows;
+    const kv::Seq s = uniform(kv::sequence(b, i));
+    const int rows = s.rows * group, row0 = tile * kWideRows + 32 * w, base = s.length - s.rows;
     const bool real = row0 + n < rows;
     const int tok = real ? (row0 + n) / group : 0;
     const int pos = real ? base + tok : -1;
     const int64_t q_row = s.first + tok, head = h * group + (real ? (row0 + n) % group : 0);
     // the positions of the wave's rows and of the block's
     const int w_first = base + min(row0, rows - 1) / group, w_last = row0 < rows ? base + (min(row0 + 32, rows) - 1) / group : -1;
-    const int b_first = base + sh_tile * kWideRows / group, b_last = base + (min((sh_tile + 1) * kWideRows, rows) - 1) / group;
+    const int b_first = base + tile * kWideRows / group, b_last = base + (min((tile + 1) * kWideRows, rows) - 1) / group;
 
     Frag q[KS][NP];
     float c;
@@ -496,87 +519,101 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
     const int per = (range.n + splits - 1) / splits, begin = min(split * per, range.n), end = min(begin + per, range.n);
     const int size = 1 << l.page_shift;
 
+    struct Pages {
+        int p[4];
+    };
+    auto pages = [&](int x) { // of the runs of a tile; what lies behind the table is behind every position too
+        Pages g;
+#pragma unroll
+        for (int y = 0; y < 4; y++) {
+            const int at = min((range.tile(x) * TT + 16 * y) >> l.page_shift, b.max_pages - 1);
+            const int page = uniform_load(b.pages + ((int64_t)i * b.max_pages + at));
+            g.p[y] = (uint32_t)page < (uint32_t)l.n_pages ? page : -1;
+        }
+        return g;
+    };
+    // Offsets of this thread's pieces: of K from its run's first byte, of V from the run's first position.  16-bit cells: of the piece whose place in LDS
+    // is the thread's.
+    constexpr int KX = 1024 / (16 * PK);                    // rows of K in a wave's 1024 bytes of LDS
+    const int k_row = w * KX + lane / PK, v_row = C::kEight ? tid / COL16 : tid / 8;
+    const int v_x = C::kEight ? tid % COL16 : (tid & 7) ^ (v_row >> 1 & 7);
+    const uint32_t k_off = C::kEight ? tid * 16 % RUN : ((k_row & 15) * D + 8 * (lane % PK ^ (PK == 16 ? k_row & 15 : k_row >> 1 & 7))) * 2;
+    const int v_run = C::kEight ? v_x : v_x >> 1;
+    const uint32_t v_off = (uint32_t)(v_row * size + (C::kEight ? 0 : 8 * (v_x & 1))) * C::kSize, v_step = (uint32_t)(kWideThreads / COL16) * size * C::kSize;
+
+    const uint32_t lds_k = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u4 *)&sh_k[0][0] + w * 1024;
+    const uint32_t lds_v = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u4 *)&sh_v[0][0] + w * 1024;
     u4 kr[LOADS], vr[LOADS];
-    int pk[LOADS], pv[LOADS], page4 = -1; // pages of the tile that is asked for next
     float scale = 0.f;
-    auto pages = [&](int x) {
+    auto load = [&](int x, const Pages &g, int buf) {
         const int t0 = range.tile(x) * TT;
+        const char *kp[4], *vp[4];
+        int64_t ph[4];
+#pragma unroll
+        for (int y = 0; y < 4; y++) {
+            ph[y] = ((int64_t)max(g.p[y], 0) * l.n_heads + h) * size;
+            const int slot = (t0 + 16 * y) & (size - 1);
+            kp[y] = (const char *)l.k + (ph[y] + slot) * D * C::kSize;
+            vp[y] = (const char *)l.v + (ph[y] * D + slot) * C::kSize;
+        }
+        const char *v_at;
+        if (size >= TT) v_at = vp[0] + 16 * C::kSize * v_run;
+        else v_at = v_run < 2 ? (v_run ? vp[1] : vp[0]) : (v_run == 2 ? vp[2] : vp[3]);
+        v_at += v_off;
 #pragma unroll
         for (int y = 0; y < LOADS; y++) {
-            const int p = tid + kWideThreads * y;
-            pk[y] = kv::page_at(b, l.n_pages, i, (t0 + p / ROW16) >> l.page_shift);
-            pv[y] = kv::page_at(b, l.n_pages, i, (t0 + (p % COL16) * (16 / C::kSize)) >> l.page_shift);
+            const int run = (w * 1024 + y * 16 * kWideThreads) / RUN;
+            const char *kb = run < 2 ? (run ? kp[1] : kp[0]) : (run == 2 ? kp[2] : kp[3]);
+            if constexpr (C::kEight) kr[y] = *(const u4 *)(kb + k_off);
+            else lds_load(lds_k + (buf * TT * PK + y * kWideThreads) * 16, kb, k_off);
         }
-        // lanes 0..63 of waves 0 and 1: the scales' pages; threads 128..131: of the four quarters
-        const int t = t0 + (tid < 128 ? tid & 63 : 16 * (tid & 3));
-        if (C::kEight || tid >= 128) page4 = kv::page_at(b, l.n_pages, i, t >> l.page_shift);
+#pragma unroll
+        for (int y = 0; y < LOADS; y++) {
+            if constexpr (C::kEight) vr[y] = *(const u4 *)(v_at + y * v_step);
+            else lds_load(lds_v + (buf * D * 8 + y * kWideThreads) * 16, v_at + y * v_step);
+        }
+        if (C::kEight && w < 2) {
+            const int run = lane >> 4;
+            const int64_t at = run < 2 ? (run ? ph[1] : ph[0]) : (run == 2 ? ph[2] : ph[3]);
+            scale = (w ? l.v_scale : l.k_scale)[at + ((t0 + lane) & (size - 1))];
+        }
     };
-    auto load = [&](int x) {
-        const int t0 = range.tile(x) * TT;
+    auto stage = [&](int buf) {
+        if constexpr (C::kEight) {
 #pragma unroll
-        for (int y = 0; y < LOADS; y++) {
-            const int p = tid + kWideThreads * y, t = t0 + p / ROW16;
-            const int64_t ph = (int64_t)max(pk[y], 0) * l.n_heads + h;
-            kr[y] = *(const u4 *)((const char *)l.k + ((ph * size + (t & (size - 1))) * D * C::kSize + 16 * (p % ROW16)));
-        }
-#pragma unroll
-        for (int y = 0; y < LOADS; y++) {
-            const int p = tid + kWideThreads * y, t = t0 + (p % COL16) * (16 / C::kSize);
-            const int64_t ph = (int64_t)max(pv[y], 0) * l.n_heads + h;
-            vr[y] = *(const u4 *)((const char *)l.v + ((ph * D + p / COL16) * size + (t & (size - 1))) * C::kSize);
-        }
-        if (C::kEight && tid < 128)
-            scale = (tid < 64 ? l.k_scale : l.v_scale)[((int64_t)max(page4, 0) * l.n_heads + h) * size + ((t0 + (tid & 63)) & (size - 1))];
-    };
-    // Whether every row of first..last sees all of a tile whose pages are there.
-    auto all_visible = [&](int t0, int first, int last) { return t0 + TT - 1 <= first && (!a.window || t0 > last - a.window || t0 + TT <= a.sinks); };
-    auto stage = [&](int x, int buf) {
-        bool odd = false;
-        if (!C::kEight && !all_visible(range.tile(x) * TT, b_first, b_last)) { // values that are not finite are added one by one (below)
-            constexpr uint32_t ones = KV == L2_KV_F16 ? 0x7C00u : 0x7F80u;
-#pragma unroll
-            for (int y = 0; y < LOADS; y++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const uint32_t v = vr[y][r];
-                    const bool lo = (v & ones) == ones, hi = (v >> 16 & ones) == ones;
-                    odd |= lo || hi;
-                    vr[y][r] = v & ((lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u));
-                }
-        }
-#pragma unroll
-        for (int y = 0; y < LOADS; y++) {
-            const int p = tid + kWideThreads * y, kr_row = p / ROW16, kr_x = p % ROW16, v_row = p / COL16, v_x = p % COL16;
-            if constexpr (C::kEight) {
+            for (int y = 0; y < LOADS; y++) {
+                const int p = tid + kWideThreads * y, kr_row = p * 16 / (D * C::kSize), kr_x = p % (D * C::kSize / 16), row = v_row + kWideThreads / COL16 * y;
                 sh_k[buf][piece_at<PK>(kr_row, 2 * kr_x)] = __builtin_bit_cast(u4, C::frag(kr[y], 0));
                 sh_k[buf][piece_at<PK>(kr_row, 2 * kr_x + 1)] = __builtin_bit_cast(u4, C::frag(kr[y], 1));
-                sh_v[buf][piece_at<8>(v_row, 2 * v_x)] = __builtin_bit_cast(u4, C::frag(vr[y], 0));
-                sh_v[buf][piece_at<8>(v_row, 2 * v_x + 1)] = __builtin_bit_cast(u4, C::frag(vr[y], 1));
-            } else {
-                // a page that is not there lies over page 0: whatever that holds is hidden, but must be finite
-                sh_k[buf][piece_at<PK>(kr_row, kr_x)] = kr[y];
-                sh_v[buf][piece_at<8>(v_row, v_x)] = pv[y] < 0 ? u4{0, 0, 0, 0} : vr[y];
+                sh_v[buf][piece_at<8>(row, 2 * v_x)] = __builtin_bit_cast(u4, C::frag(vr[y], 0));
+                sh_v[buf][piece_at<8>(row, 2 * v_x + 1)] = __builtin_bit_cast(u4, C::frag(vr[y], 1));
             }
+            if (w < 2) (w ? sh_vs : sh_ks)[buf][lane] = scale;
+        } else {
+            wait_lds_loads();
         }
-        if (C::kEight && tid < 128) (tid < 64 ? sh_ks : sh_vs)[buf][tid & 63] = scale;
-        if (tid >= 128 && tid < 132) sh_page[buf][tid & 3] = page4;
-        if (odd) sh_odd[buf] = x;
     };
+    // Whether every row of the wave sees all of a tile whose pages are there.
+    auto all_visible = [&](int t0) { return t0 + TT - 1 <= w_first && (!a.window || t0 > w_last - a.window || t0 + TT <= a.sinks); };
 
     f16v acc[DT] = {};
     float top = -kInf, e = kLeastE, off = -kInf, sum = 0.f;
+    Pages here{}, next{};
     if (begin < end) {
-        pages(begin);
-        load(begin);
-        stage(begin, 0);
+        here = pages(begin);
+        load(begin, here, 0);
+        if (begin + 1 < end) next = pages(begin + 1);
+        stage(0);
         __syncthreads();
     }
     for (int x = begin; x < end; x++) {
         const int buf = (x - begin) & 1, t0 = range.tile(x) * TT;
         const bool more = x + 1 < end;
+        const Pages now_here = here;
         if (more) {
-            pages(x + 1);
-            load(x + 1);
+            load(x + 1, next, buf ^ 1);
+            here = next;
+            if (x + 2 < end) next = pages(x + 2);
         }
         const bool none = w_last < t0 || (a.window && t0 + TT - 1 <= w_first - a.window && t0 >= a.sinks);
         if (!none) {
@@ -591,8 +628,7 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
 #pragma unroll
                     for (int z = 0; z < NP; z++) sc[y] = mfma32(f, q[k][z], sc[y]);
                 }
-            const bool there = sh_page[buf][0] >= 0 && sh_page[buf][1] >= 0 && sh_page[buf][2] >= 0 && sh_page[buf][3] >= 0;
-            const bool whole = there && all_visible(t0, w_first, w_last);
+            const bool whole = (now_here.p[0] | now_here.p[1] | now_here.p[2] | now_here.p[3]) >= 0 && all_visible(t0);
             f4 vs[8];
             if (C::kEight) {
 #pragma unroll
@@ -608,7 +644,7 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
 #pragma unroll
                 for (int z = 0; z < 8; z++) {
                     const int t = 32 * (z / 4) + 16 * (z / 2 & 1) + 8 * hh + 4 * (z & 1);
-                    const bool here = sh_page[buf][t >> 4] >= 0;
+                    const bool here = now_here.p[2 * (z / 4) + (z / 2 & 1)] >= 0; // t / 16
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         const bool see = here && visible(a, t0 + t + r, pos);
@@ -640,6 +676,7 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
                 sum *= f;
             }
             off = top == -kInf ? -kInf : now;
+            bool odd = false; // a value that is not finite where some row may not see it
 #pragma unroll
             for (int v = 0; v < 4; v++) { // positions 16 v + 8 hh + j
                 f8 p;
@@ -654,28 +691,34 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
                 pieces<Frag, typename C::One, NP>(p, pf);
 #pragma unroll
                 for (int y = 0; y < DT; y++) {
-                    const Frag fr = __builtin_bit_cast(Frag, sh_v[buf][piece_at<8>(32 * y + n, 2 * v + hh)]);
+                    u4 bits = sh_v[buf][piece_at<8>(32 * y + n, 2 * v + hh)];
+                    if (!C::kEight && !whole) bits = finite<KV>(bits, odd);
+                    const Frag fr = __builtin_bit_cast(Frag, bits);
 #pragma unroll
                     for (int z = 0; z < NP; z++) acc[y] = mfma32(fr, pf[z], acc[y]);
                 }
             }
-            if (!C::kEight && sh_odd[buf] == x) {
+            if (!C::kEight && __ballot(odd)) { // added one by one, to the rows that see them
+                const uint16_t *cells = (const uint16_t *)&sh_v[buf][0];
+#pragma unroll 1
                 for (int y = 0; y < TT; y++) {
-                    const int t = t0 + y, page = kv::page_at(b, l.n_pages, i, t >> l.page_shift);
-                    if (page < 0 || !visible(a, t, pos)) continue;
-                    const uint16_t *p = (const uint16_t *)l.v + (((int64_t)page * l.n_heads + h) * D * size + (t & (size - 1)));
+                    const int page = y < 32 ? (y < 16 ? now_here.p[0] : now_here.p[1]) : (y < 48 ? now_here.p[2] : now_here.p[3]);
+                    if (page < 0 || !visible(a, t0 + y, pos)) continue;
 #pragma unroll
-                    for (int z = 0; z < DT; z++)
+                    for (int z = 0; z < DT; z++) {
 #pragma unroll
                         for (int r = 0; r < 16; r++) {
-                            const uint16_t bits = p[(int64_t)(32 * z + 8 * (r / 4) + 4 * hh + r % 4) * size];
+                            const int d = 32 * z + 8 * (r / 4) + 4 * hh + r % 4;
+                            const uint16_t bits = cells[8 * piece_at<8>(d, y >> 3) + (y & 7)];
                             const float v = KV == L2_KV_F16 ? (float)__builtin_bit_cast(_Float16, bits) : kv::bf16_float(bits);
                             if (!(fabsf(v) < kInf)) acc[z][r] += v;
                         }
+                        asm volatile("" ::: "memory");
+                    }
                 }
             }
         }
-        if (more) stage(x + 1, buf ^ 1);
+        if (more) stage(buf ^ 1);
         __syncthreads();
     }
     const lanes::Both s2 = lanes::both32(sum);
