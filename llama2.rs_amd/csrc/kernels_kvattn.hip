@@ -5,10 +5,11 @@
 // the fitting order; maxima and sums are a lane's own but for two exchanges, and the factors between tiles one register.  V lies transposed in the pool, so
 // nothing is transposed here.  Codes of 8 bits become 16-bit floats exactly (fp16).  Scales of keys multiply the scores, those of values the weights.
 //
-// Weights enter the second product in 16 bits, fp16 as 2^15 at most: p_t = exp2(s_t - off) with off = max s + e - 15, where 2^e is the power of two above the largest
-// scale of the values seen; then p_t * (scale of v_t) is below 2^15 whatever the scales, and off cancels in the quotient with the sum of the p_t.  fp32 rows have q
-// and p in two fp16 numbers (2^-22) or, over a pool in bf16, in three; rows of 16 bits in one where that holds a q as it is.  q is scaled by a power of two per
-// row, so that fp16 holds what bf16 and fp32 rows may contain.
+// Weights enter the second product in 16 bits, times a factor that cancels in the quotient with their sum: p_t = exp2(s_t - off).  `off` follows the tiles' max s + e, where
+// 2^e is the power of two above the largest scale of their values, so that p_t * (scale of v_t) is what is bounded, by 2^15 for fp16: off goes to 7 below max s + e, and
+// is left where it is until that lies more than 8 higher, so that sums are seldom rescaled (a tile of 32 rows would have a new maximum among them nearly always).
+// fp32 rows have q and p in two fp16 numbers (2^-22; a weight that is 2^-21 of the largest or less, to within 2^-32 of the largest) or, over a pool in
+// bf16, in three; rows of 16 bits in one where that holds a q as it is.  q is scaled by a power of two per row, so that fp16 holds what bf16 and fp32 rows may contain.
 #include <algorithm>
 
 #include "kvpool.h"
@@ -26,6 +27,18 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLeastE = -67.f; // rows whose values are held at all have scales from 2^-67
+constexpr float kBase = 7.f, kSlack = 8.f;
+
+// `off` behind a tile whose largest score times its factor is `top`, and the factor of the sums so far.
+__device__ __forceinline__ float follow(float &off, float top) {
+    const float to = top - kBase;
+    if (!(to > off + kSlack)) return 1.f; // or nothing is seen
+    const float f = __builtin_amdgcn_exp2f(off - to);
+    off = to;
+    return f;
+}
+// 2^e above x.
+__device__ __forceinline__ float above(float x) { return x > 0.f ? fmaxf((float)__builtin_amdgcn_frexp_expf(x), kLeastE) : kLeastE; }
 
 // What a pool's cells become for the matrix cores: eight of them, from 8 (16) bytes.
 template <int KV>
@@ -156,7 +169,7 @@ struct Parts {
 // four waves tiles of 64 positions (32 of 16-bit cells) in turn, straight from memory into registers: 8 KB of keys and 8 KB of values, the next tile's keys
 // asked for once this one's scores are there and its values once this one's are summed.
 template <int KV, int NP, int D>
-__global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, int splits, int stride) {
+__global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, int splits, int stride, int narrow) {
     using C = Cells<KV>;
     using Frag = typename C::Frag;
     constexpr int TT = 64 / C::kSize, ST = TT / 16, CH = TT / 4, FR = 2 / C::kSize, KL = D * C::kSize / 64, DT = D / 16, VS = TT / 32;
@@ -164,7 +177,7 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
     const kv::Seq s = kv::sequence(b, i);
     const int group = a.n_heads / l.n_heads, rows = s.rows * group;
-    if (rows == 0 || rows > kNarrowRows) return;
+    if (rows == 0 || rows > narrow) return;
     const int base = s.length - s.rows; // position of the first row
     const bool real = m < rows;
     const int pos = real ? base + m / group : -1;
@@ -239,7 +252,7 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
     };
 
     f4 acc[DT] = {};
-    float top = -kInf, e = kLeastE, off = -kInf, sum = 0.f;
+    float off = -kInf, sum = 0.f;
     int n = begin + w;
     if (n < end) {
         pages(n);
@@ -287,25 +300,22 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
         for (int x = 0; x < ST; x++)
 #pragma unroll
             for (int r = 0; r < 4; r++) mx = fmaxf(mx, sc[x][r]);
-        top = fmaxf(top, lanes::rows_max(mx) * c);
+        float top = lanes::rows_max(mx) * c;
         if (C::kEight) {
             float mv = 0.f;
 #pragma unroll
             for (int x = 0; x < ST; x++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) mv = fmaxf(mv, vs[x][r]);
-            mv = lanes::rows_max(mv);
-            if (mv > 0.f) e = fmaxf(e, (float)__builtin_amdgcn_frexp_expf(mv));
+            top += above(lanes::rows_max(mv));
         }
-        // nothing seen yet: every weight is exp2(-inf)
-        const float now = top == -kInf ? 0.f : C::kEight ? top + (e - 15.f) : C::kHalf ? top - 15.f : top;
-        const float f = off == now ? 1.f : __builtin_amdgcn_exp2f(off - now);
+        const float f = follow(off, top);
         if (__ballot(f != 1.f)) {
 #pragma unroll
             for (int x = 0; x < DT; x++) acc[x] *= f;
             sum *= f;
         }
-        off = top == -kInf ? -kInf : now;
+        const float now = off == -kInf ? 0.f : off; // nothing seen yet: every weight is exp2(-inf)
 #pragma unroll
         for (int v = 0; v < VS; v++) {
             f8 p;
@@ -382,16 +392,15 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
     }
 }
 
-// Joins the splits of each query row: one wave per row and head.
-template <int D>
-__global__ __launch_bounds__(64) void kv_join_kernel(l2_kvbatch b, KvAttention a, Parts parts, int narrow, int wide, int stride, int group) {
-    const int row = blockIdx.x, hq = blockIdx.y, lane = threadIdx.x;
-    const int i = kv::sequence_of(b, row);
+// Joins the parts of each query row: one wave per row and head.  NARROW: block x has row x % most of sequence x / most, most rows at the most; else row x.
+template <int D, bool NARROW>
+__global__ __launch_bounds__(64) void kv_join_kernel(l2_kvbatch b, KvAttention a, Parts parts, int splits, int stride, int group, int most) {
+    const int hq = blockIdx.y, lane = threadIdx.x;
+    const int i = NARROW ? (int)blockIdx.x / most : kv::sequence_of(b, blockIdx.x);
     if (i >= b.n_seqs) return;
     const kv::Seq s = kv::sequence(b, i);
-    if (row - s.first >= s.rows) return;
-    const int splits = (int64_t)s.rows * group > kNarrowRows ? wide : narrow;
-    if (splits == 1) return;
+    const int row = NARROW ? s.first + (int)blockIdx.x % most : blockIdx.x;
+    if (row - s.first >= s.rows || ((int64_t)s.rows * group <= most * group) != NARROW) return;
     const int64_t at = ((int64_t)row * a.n_heads + hq) * stride;
     float o = -kInf, total = 0.f;
     for (int x = 0; x < splits; x++) o = fmaxf(o, parts.stat[at + x].x);
@@ -419,6 +428,12 @@ __device__ __forceinline__ int piece_at(int r, int x) {
     return r * PER_ROW + (PER_ROW == 16 ? x ^ (r & 15) : x ^ (r >> 1 & 7));
 }
 
+__device__ __forceinline__ float wave_max(float v) {
+    v = lanes::rows_max(v);
+    for (int o = 8; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+
 // Values that are the same in every lane, in scalar registers.
 __device__ __forceinline__ kv::Seq uniform(const kv::Seq &s) {
     return {__builtin_amdgcn_readfirstlane(s.first), __builtin_amdgcn_readfirstlane(s.rows), __builtin_amdgcn_readfirstlane(s.length)};
@@ -442,7 +457,7 @@ __device__ __forceinline__ void wait_lds_loads() { asm volatile("s_waitcnt vmcnt
 // bits, the next tile on its way meanwhile: codes of 8 bits into registers, to be converted once for all four waves, 16-bit cells straight into LDS.  A tile is
 // four runs of 16 positions, each in one page; their addresses are computed once per wave.
 template <int KV, int NP, int D>
-__global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, int splits, int stride) {
+__global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, int splits, int stride, int narrow) {
     using C = Cells<KV>;
     using Frag = typename C::Frag;
     constexpr int TT = 64, PK = D / 8, DT = D / 32, KS = D / 16, LOADS = TT * D * C::kSize / 16 / kWideThreads;
@@ -450,10 +465,11 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
     constexpr int COL16 = TT * C::kSize / 16;     // 16-byte pieces of the tile's part of a row of V
     __shared__ __align__(16) u4 sh_k[2][TT * PK], sh_v[2][D * 8];
     __shared__ __align__(16) float sh_ks[2][TT], sh_vs[2][TT];
+    __shared__ float sh_top[2];
     __shared__ int sh_seq, sh_tile;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, hh = lane >> 5;
     const int group = a.n_heads / l.n_heads;
-    const int h = blockIdx.x % l.n_heads, split = blockIdx.x / l.n_heads % splits;
+    const int h = __builtin_amdgcn_readfirstlane(blockIdx.x % l.n_heads), split = __builtin_amdgcn_readfirstlane(blockIdx.x / l.n_heads % splits);
 
     // which sequence's rows: the tiles of all sequences one behind the other
     {
@@ -464,7 +480,7 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
             int tiles = 0;
             if (i0 + lane < b.n_seqs) {
                 const int64_t r = (int64_t)kv::sequence(b, i0 + lane).rows * group;
-                tiles = r > kNarrowRows ? (int)((r + kWideRows - 1) / kWideRows) : 0;
+                tiles = r > narrow ? (int)((r + kWideRows - 1) / kWideRows) : 0;
             }
             int upto = tiles;
             for (int o = 1; o < 64; o <<= 1) {
@@ -487,8 +503,10 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
     const int pos = real ? base + tok : -1;
     const int64_t q_row = s.first + tok, head = h * group + (real ? (row0 + n) % group : 0);
     // the positions of the wave's rows and of the block's
-    const int w_first = base + min(row0, rows - 1) / group, w_last = row0 < rows ? base + (min(row0 + 32, rows) - 1) / group : -1;
-    const int b_first = base + tile * kWideRows / group, b_last = base + (min((tile + 1) * kWideRows, rows) - 1) / group;
+    const int w_first = __builtin_amdgcn_readfirstlane(base + min(row0, rows - 1) / group);
+    const int w_last = __builtin_amdgcn_readfirstlane(row0 < rows ? base + (min(row0 + 32, rows) - 1) / group : -1);
+    const int b_first = __builtin_amdgcn_readfirstlane(base + tile * kWideRows / group);
+    const int b_last = __builtin_amdgcn_readfirstlane(base + (min((tile + 1) * kWideRows, rows) - 1) / group);
 
     Frag q[KS][NP];
     float c;
@@ -516,7 +534,7 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
     }
 
     const Range range = range_of<TT>(a, b_first, b_last);
-    const int per = (range.n + splits - 1) / splits, begin = min(split * per, range.n), end = min(begin + per, range.n);
+    const int per = __builtin_amdgcn_readfirstlane((range.n + splits - 1) / splits), begin = min(split * per, range.n), end = min(begin + per, range.n);
     const int size = 1 << l.page_shift;
 
     struct Pages {
@@ -589,6 +607,10 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
                 sh_v[buf][piece_at<8>(row, 2 * v_x + 1)] = __builtin_bit_cast(u4, C::frag(vr[y], 1));
             }
             if (w < 2) (w ? sh_vs : sh_ks)[buf][lane] = scale;
+            if (w == 1) {
+                const float most = wave_max(scale);
+                if (lane == 0) sh_top[buf] = most;
+            }
         } else {
             wait_lds_loads();
         }
@@ -597,7 +619,7 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
     auto all_visible = [&](int t0) { return t0 + TT - 1 <= w_first && (!a.window || t0 > w_last - a.window || t0 + TT <= a.sinks); };
 
     f16v acc[DT] = {};
-    float top = -kInf, e = kLeastE, off = -kInf, sum = 0.f;
+    float off = -kInf, sum = 0.f;
     Pages here{}, next{};
     if (begin < end) {
         here = pages(begin);
@@ -629,53 +651,52 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
                     for (int z = 0; z < NP; z++) sc[y] = mfma32(f, q[k][z], sc[y]);
                 }
             const bool whole = (now_here.p[0] | now_here.p[1] | now_here.p[2] | now_here.p[3]) >= 0 && all_visible(t0);
-            f4 vs[8];
+            auto run_of = [](int z) { return 32 * (z / 4) + 16 * (z / 2 & 1) + 4 * (z & 1); }; // of element 4 (z & 3) of sc[z / 4], less 8 hh
             if (C::kEight) {
 #pragma unroll
                 for (int z = 0; z < 8; z++) {
-                    const int t = 32 * (z / 4) + 16 * (z / 2 & 1) + 8 * hh + 4 * (z & 1);
-                    const f4 ks = *(const f4 *)&sh_ks[buf][t];
-                    vs[z] = *(const f4 *)&sh_vs[buf][t];
+                    const f4 ks = *(const f4 *)&sh_ks[buf][run_of(z) + 8 * hh];
 #pragma unroll
                     for (int r = 0; r < 4; r++) sc[z / 4][4 * (z & 3) + r] *= ks[r];
                 }
             }
-            if (!whole) {
+            float top_v = 0.f; // the largest scale of the values that the row sees
+            if (whole) {
+                if (C::kEight) top_v = sh_top[buf];
+            } else {
 #pragma unroll
                 for (int z = 0; z < 8; z++) {
-                    const int t = 32 * (z / 4) + 16 * (z / 2 & 1) + 8 * hh + 4 * (z & 1);
+                    const int t = run_of(z) + 8 * hh;
                     const bool here = now_here.p[2 * (z / 4) + (z / 2 & 1)] >= 0; // t / 16
+                    f4 vs = {};
+                    if (C::kEight) vs = *(const f4 *)&sh_vs[buf][t];
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         const bool see = here && visible(a, t0 + t + r, pos);
                         sc[z / 4][4 * (z & 3) + r] = see ? sc[z / 4][4 * (z & 3) + r] : -kInf;
-                        if (C::kEight) vs[z][r] = see ? vs[z][r] : 0.f;
+                        if (C::kEight) top_v = fmaxf(top_v, see ? vs[r] : 0.f);
                     }
                 }
+                if (C::kEight) {
+                    const lanes::Both v2 = lanes::both32(top_v);
+                    top_v = fmaxf(v2.lo, v2.hi);
+                }
             }
-            float mx = -kInf, mv = 0.f;
+            float mx = -kInf;
 #pragma unroll
             for (int z = 0; z < 8; z++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    mx = fmaxf(mx, sc[z / 4][4 * (z & 3) + r]);
-                    if (C::kEight) mv = fmaxf(mv, vs[z][r]);
-                }
+                for (int r = 0; r < 4; r++) mx = fmaxf(mx, sc[z / 4][4 * (z & 3) + r]);
             const lanes::Both m2 = lanes::both32(mx);
-            top = fmaxf(top, fmaxf(m2.lo, m2.hi) * c);
-            if (C::kEight) {
-                const lanes::Both v2 = lanes::both32(mv);
-                mv = fmaxf(v2.lo, v2.hi);
-                if (mv > 0.f) e = fmaxf(e, (float)__builtin_amdgcn_frexp_expf(mv));
-            }
-            const float now = top == -kInf ? 0.f : C::kEight ? top + (e - 15.f) : C::kHalf ? top - 15.f : top;
-            const float f = off == now ? 1.f : __builtin_amdgcn_exp2f(off - now);
+            float top = fmaxf(m2.lo, m2.hi) * c;
+            if (C::kEight) top += above(top_v);
+            const float f = follow(off, top);
             if (__ballot(f != 1.f)) {
 #pragma unroll
                 for (int y = 0; y < DT; y++) acc[y] *= f;
                 sum *= f;
             }
-            off = top == -kInf ? -kInf : now;
+            const float now = off == -kInf ? 0.f : off; // nothing seen yet: every weight is exp2(-inf)
             bool odd = false; // a value that is not finite where some row may not see it
 #pragma unroll
             for (int v = 0; v < 4; v++) { // positions 16 v + 8 hh + j
@@ -683,9 +704,16 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const int z = 2 * v + j / 4;
-                    const float t = __builtin_amdgcn_exp2f(fmaf(sc[z / 4][4 * (z & 3) + j % 4], c, -now));
-                    sum += t;
-                    p[j] = C::kEight ? t * vs[z][j % 4] : t;
+                    p[j] = __builtin_amdgcn_exp2f(fmaf(sc[z / 4][4 * (z & 3) + j % 4], c, -now));
+                    sum += p[j];
+                }
+                if (C::kEight) {
+                    const f4 v0 = *(const f4 *)&sh_vs[buf][16 * v + 8 * hh], v1 = *(const f4 *)&sh_vs[buf][16 * v + 8 * hh + 4];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) p[j] *= j < 4 ? v0[j % 4] : v1[j % 4];
+                    if (!whole) // the scale of a row that is not seen may be NaN
+#pragma unroll
+                        for (int j = 0; j < 8; j++) p[j] = sc[v / 2][8 * (v & 1) + j] == -kInf ? 0.f : p[j];
                 }
                 Frag pf[NP];
                 pieces<Frag, typename C::One, NP>(p, pf);
@@ -747,14 +775,14 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
     }
 }
 
-typedef void (*AttnKernel)(KvLayer, l2_kvbatch, KvAttention, Parts, int, int);
+typedef void (*AttnKernel)(KvLayer, l2_kvbatch, KvAttention, Parts, int, int, int);
 #define SIZES(kernel, kv, np) {kernel<kv, np, 64>, kernel<kv, np, 128>}
 #define ALL(kernel)                                                                                                                             \
     {{SIZES(kernel, 0, 1), SIZES(kernel, 0, 2), {}}, {SIZES(kernel, 1, 1), SIZES(kernel, 1, 2), {}}, {SIZES(kernel, 2, 1), SIZES(kernel, 2, 2), {}}, \
      {SIZES(kernel, 3, 1), SIZES(kernel, 3, 2), SIZES(kernel, 3, 3)}}
 const AttnKernel kNarrow[4][3][2] = ALL(kv_narrow_kernel), kWide[4][3][2] = ALL(kv_wide_kernel);
 typedef void (*JoinKernel)(l2_kvbatch, KvAttention, Parts, int, int, int, int);
-const JoinKernel kJoin[2] = {kv_join_kernel<64>, kv_join_kernel<128>};
+const JoinKernel kJoin[2][2] = {{kv_join_kernel<64, false>, kv_join_kernel<64, true>}, {kv_join_kernel<128, false>, kv_join_kernel<128, true>}};
 
 // In how many 16-bit numbers q and the weights enter the matrix cores, less one.
 int pieces_index(int kv_type, int type) {
@@ -775,15 +803,19 @@ void kv_attention_plan(const KvLayer &l, int kv_type, const l2_kvbatch &b, const
     auto parts_of = [&](int64_t blocks, int64_t full, int64_t tiles, int64_t least) {
         return (int)std::max<int64_t>(1, std::min<int64_t>((full + blocks - 1) / blocks, tiles / least));
     };
-    plan->narrow = group <= kNarrowRows;
     plan->wide = rows * group > kNarrowRows;
+    // A single sequence is the one kernel's or the other's; several may be some of each.
+    plan->narrow_rows = group > kNarrowRows || (plan->wide && seqs == 1) ? 0 : kNarrowRows / group * group;
     plan->narrow_splits = plan->wide_splits = 1;
-    if (plan->narrow)
+    if (plan->narrow_rows)
         plan->narrow_splits = parts_of(seqs * l.n_heads, 2 * cu_count(), tiles_seen(kv_type <= L2_KV_E4M3 ? 64 : 32, kNarrowRows), 2 * kNarrowWaves);
     // row tiles of all sequences, at most: their whole ones, and a last one of each that has more rows than the narrow kernel takes
     const int64_t all = (int64_t)b.n_rows * group;
-    plan->wide_tiles = (int)std::min<int64_t>(all / kWideRows + std::min<int64_t>(seqs, all / (kNarrowRows + 1)), 1 << 26);
-    if (plan->wide) plan->wide_splits = parts_of(std::max<int64_t>(plan->wide_tiles, 1) * l.n_heads, cu_count(), tiles_seen(64, (kWideRows + group - 1) / group), 4);
+    plan->wide_tiles = (int)std::min<int64_t>(all / kWideRows + std::min<int64_t>(seqs, all / (plan->narrow_rows + 1)), 1 << 26);
+    // blocks for every CU's room: two, or one of those with more registers
+    const int room = pieces_index(kv_type, a.type) == 0 ? 2 : 1;
+    if (plan->wide)
+        plan->wide_splits = parts_of(std::max<int64_t>(all / kWideRows, 1) * l.n_heads, room * cu_count(), tiles_seen(64, (kWideRows + group - 1) / group), 4);
     plan->stride = std::max(plan->narrow_splits, plan->wide_splits);
     plan->workspace = plan->stride > 1 ? (size_t)b.n_rows * a.n_heads * plan->stride * (l.head_size * 4 + 8) : 0;
 }
@@ -796,12 +828,18 @@ int kv_attention_launch(const KvLayer &l, int kv_type, const l2_kvbatch &b, cons
     if (plan.wide && plan.wide_tiles) {
         const int64_t blocks = (int64_t)plan.wide_tiles * l.n_heads * plan.wide_splits;
         if (blocks >= (int64_t)1 << 31) return l2_fail(L2_ERR_RANGE, "%d rows of %d heads", b.n_rows, a.n_heads);
-        l2_launch(kWide[kv_type][np][big], dim3((unsigned)blocks), dim3(kWideThreads), 0, st, l, b, a, parts, plan.wide_splits, plan.stride);
+        l2_launch(kWide[kv_type][np][big], dim3((unsigned)blocks), dim3(kWideThreads), 0, st, l, b, a, parts, plan.wide_splits, plan.stride,
+                  plan.narrow_rows);
     }
-    if (plan.narrow)
+    if (plan.narrow_rows)
         l2_launch(kNarrow[kv_type][np][big], dim3(plan.narrow_splits, l.n_heads, b.n_seqs), dim3(64 * kNarrowWaves), 0, st, l, b, a, parts, plan.narrow_splits,
-                  plan.stride);
-    if (plan.stride > 1) l2_launch(kJoin[big], dim3(b.n_rows, a.n_heads), dim3(64), 0, st, b, a, parts, plan.narrow_splits, plan.wide_splits, plan.stride, group);
+                  plan.stride, plan.narrow_rows);
+    const int most = plan.narrow_rows / group; // rows of a sequence that the narrow kernel takes
+    if (plan.narrow_rows && plan.narrow_splits > 1)
+        l2_launch(kJoin[big][1], dim3(b.n_seqs * std::min(most, b.max_rows), a.n_heads), dim3(64), 0, st, b, a, parts, plan.narrow_splits, plan.stride, group,
+                  std::min(most, b.max_rows));
+    if (plan.wide && plan.wide_splits > 1)
+        l2_launch(kJoin[big][0], dim3(b.n_rows, a.n_heads), dim3(64), 0, st, b, a, parts, plan.wide_splits, plan.stride, group, most);
     L2_HIP(hipGetLastError());
     return L2_OK;
 }
@@ -813,6 +851,6 @@ int kv_attention_warm_up() {
             for (auto &n : k)
                 for (AttnKernel f : n)
                     if (f) L2_HIP(hipFuncGetAttributes(&a, (const void *)f));
-    for (JoinKernel f : kJoin) L2_HIP(hipFuncGetAttributes(&a, (const void *)f));
+    for (auto &k : kJoin) for (JoinKernel f : k) L2_HIP(hipFuncGetAttributes(&a, (const void *)f));
     return L2_OK;
 }

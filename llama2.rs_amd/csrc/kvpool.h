@@ -37,7 +37,8 @@ struct KvAttention {
 // How the limits of a call are cut up: a function of them alone.
 struct KvAttnPlan {
     size_t workspace;               // bytes
-    bool narrow, wide;              // which kernels there may be sequences for
+    bool wide;                      // whether there may be sequences of more rows than ..
+    int narrow_rows;                // .. the narrow kernel takes, per kv head; 0: it takes none
     int narrow_splits, wide_splits; // parts that positions are cut into
     int stride;                     // the larger of both: parts of a row in the workspace
     int wide_tiles;                 // tiles of rows of the wide kernel, at most
