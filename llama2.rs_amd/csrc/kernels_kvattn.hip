@@ -335,15 +335,18 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
             }
         }
         if (__ballot(odd)) { // added one by one, to the rows that see them
+#pragma unroll 1
             for (int y = 0; y < TT; y++) {
                 const int t = t0 + y, page = kv::page_at(b, l.n_pages, i, t >> l.page_shift);
                 if (page < 0 || !visible(a, t, pos)) continue;
+                int first = 4 * g; // unknown, so that the places are not worked out ahead of the loop
+                asm volatile("" : "+v"(first));
                 const uint16_t *p = (const uint16_t *)vb + (((int64_t)page * l.n_heads + h) * D * size + (t & (size - 1)));
 #pragma unroll
                 for (int x = 0; x < DT; x++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const uint16_t bits = p[(int64_t)(16 * x + 4 * g + r) * size];
+                        const uint16_t bits = p[(int64_t)(16 * x + first + r) * size];
                         const float v = KV == L2_KV_F16 ? (float)__builtin_bit_cast(_Float16, bits) : kv::bf16_float(bits);
                         if (!(fabsf(v) < kInf)) acc[x][r] += v;
                     }
@@ -732,11 +735,13 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
                 for (int y = 0; y < TT; y++) {
                     const int page = y < 32 ? (y < 16 ? now_here.p[0] : now_here.p[1]) : (y < 48 ? now_here.p[2] : now_here.p[3]);
                     if (page < 0 || !visible(a, t0 + y, pos)) continue;
+                    int half = hh; // unknown, so that 64 places are not worked out ahead of the loop
+                    asm volatile("" : "+v"(half));
 #pragma unroll
                     for (int z = 0; z < DT; z++) {
 #pragma unroll
                         for (int r = 0; r < 16; r++) {
-                            const int d = 32 * z + 8 * (r / 4) + 4 * hh + r % 4;
+                            const int d = 32 * z + 8 * (r / 4) + 4 * half + r % 4;
                             const uint16_t bits = cells[8 * piece_at<8>(d, y >> 3) + (y & 7)];
                             const float v = KV == L2_KV_F16 ? (float)__builtin_bit_cast(_Float16, bits) : kv::bf16_float(bits);
                             if (!(fabsf(v) < kInf)) acc[z][r] += v;
