@@ -20,8 +20,8 @@ namespace {
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-typedef float f4 __attribute__((ext_vector_type(4)));
-typedef float f8 __attribute__((ext_vector_type(8)));
+using kv::f4;
+using kv::f8;
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr float kInf = __builtin_inff();
@@ -97,33 +97,6 @@ __device__ __forceinline__ void pieces(f8 x, Frag (&out)[NP]) {
     }
 }
 
-// Eight values of a row of the caller's, aligned as their type is.
-__device__ __forceinline__ f8 load8(const void *p, int type, int64_t i) {
-    typedef float any __attribute__((ext_vector_type(8), aligned(4)));
-    typedef _Float16 anyh __attribute__((ext_vector_type(8), aligned(2)));
-    typedef uint16_t anyb __attribute__((ext_vector_type(8), aligned(2)));
-    f8 x;
-    if (type == L2_F32) {
-        const any v = *(const any *)((const float *)p + i);
-        for (int j = 0; j < 8; j++) x[j] = v[j];
-    } else if (type == L2_F16) {
-        const anyh v = *(const anyh *)((const _Float16 *)p + i);
-        for (int j = 0; j < 8; j++) x[j] = (float)v[j];
-    } else {
-        const anyb v = *(const anyb *)((const uint16_t *)p + i);
-        for (int j = 0; j < 8; j++) x[j] = kv::bf16_float(v[j]);
-    }
-    return x;
-}
-
-__device__ __forceinline__ void store4(void *p, int type, int64_t i, const f4 &v) {
-    typedef _Float16 anyh __attribute__((ext_vector_type(4), aligned(2)));
-    typedef uint16_t anyb __attribute__((ext_vector_type(4), aligned(2)));
-    if (type == L2_F32) *(float4_any *)((float *)p + i) = float4_any{v[0], v[1], v[2], v[3]};
-    else if (type == L2_F16) *(anyh *)((_Float16 *)p + i) = anyh{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
-    else *(anyb *)((uint16_t *)p + i) = anyb{kv::float_bf16(v[0]), kv::float_bf16(v[1]), kv::float_bf16(v[2]), kv::float_bf16(v[3])};
-}
-
 // The positions that the rows of a tile of queries have to do with, in tiles of TT: those of the first tokens that stay visible, then those from the
 // first row's window (or from the start) to the last row's own.
 struct Range {
@@ -192,7 +165,7 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
 #pragma unroll
         for (int k = 0; k < D / 32; k++) {
             const int d = (k / FR) * (64 / C::kSize) + (16 / C::kSize) * g + 8 * (k % FR);
-            x[k] = load8(a.q, a.type, q_row * a.q_stride + head * D + d);
+            x[k] = kv::load8(a.q, a.type, q_row * a.q_stride + head * D + d);
 #pragma unroll
             for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[k][j]));
         }
@@ -386,7 +359,7 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
         if (splits == 1) {
             const float inv = total == 0.f ? 0.f : 1.f / total;
             for (int j = 0; j < 4; j++) v[j] = total == 0.f ? 0.f : v[j] * inv;
-            store4(a.out, a.type, row * a.out_stride + hq * D + d, v);
+            kv::store4(a.out, a.type, row * a.out_stride + hq * D + d, v);
         } else {
             const int64_t at = (row * a.n_heads + hq) * stride + split;
             *(f4 *)(parts.acc + at * D + d) = v;
@@ -519,7 +492,7 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
         int e = 0;
         if (C::kHalf) {
             for (int k = 0; k < KS; k++) {
-                const f8 x = load8(a.q, a.type, q_row * a.q_stride + head * D + 16 * k + 8 * hh);
+                const f8 x = kv::load8(a.q, a.type, q_row * a.q_stride + head * D + 16 * k + 8 * hh);
                 for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[j]));
             }
             const lanes::Both t = lanes::both32(top);
@@ -529,7 +502,7 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
         }
 #pragma unroll
         for (int k = 0; k < KS; k++) {
-            f8 x = load8(a.q, a.type, q_row * a.q_stride + head * D + 16 * k + 8 * hh);
+            f8 x = kv::load8(a.q, a.type, q_row * a.q_stride + head * D + 16 * k + 8 * hh);
             if (C::kHalf)
                 for (int j = 0; j < 8; j++) x[j] = ldexpf(x[j], e);
             pieces<Frag, typename C::One, NP>(x, q[k]);
@@ -767,7 +740,7 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
                 f4 v;
 #pragma unroll
                 for (int r = 0; r < 4; r++) v[r] = sum == 0.f ? 0.f : acc[y][4 * z + r] * inv;
-                store4(a.out, a.type, at, v);
+                kv::store4(a.out, a.type, at, v);
             }
     } else {
         const int64_t at = (q_row * a.n_heads + head) * stride + split;

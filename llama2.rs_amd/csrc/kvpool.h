@@ -99,5 +99,47 @@ __device__ __forceinline__ void store(void *p, int type, int64_t i, float v) {
     else ((uint16_t *)p)[i] = float_bf16(v);
 }
 
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f8 __attribute__((ext_vector_type(8)));
+
+// Eight values of a row of the caller's, aligned as their type is.
+__device__ __forceinline__ f8 load8(const void *p, int type, int64_t i) {
+    typedef float any __attribute__((ext_vector_type(8), aligned(4)));
+    typedef _Float16 anyh __attribute__((ext_vector_type(8), aligned(2)));
+    typedef uint16_t anyb __attribute__((ext_vector_type(8), aligned(2)));
+    f8 x;
+    if (type == L2_F32) {
+        const any v = *(const any *)((const float *)p + i);
+        for (int j = 0; j < 8; j++) x[j] = v[j];
+    } else if (type == L2_F16) {
+        const anyh v = *(const anyh *)((const _Float16 *)p + i);
+        for (int j = 0; j < 8; j++) x[j] = (float)v[j];
+    } else {
+        const anyb v = *(const anyb *)((const uint16_t *)p + i);
+        for (int j = 0; j < 8; j++) x[j] = bf16_float(v[j]);
+    }
+    return x;
+}
+
+__device__ __forceinline__ void store4(void *p, int type, int64_t i, const f4 &v) {
+    typedef _Float16 anyh __attribute__((ext_vector_type(4), aligned(2)));
+    typedef uint16_t anyb __attribute__((ext_vector_type(4), aligned(2)));
+    if (type == L2_F32) *(float4_any *)((float *)p + i) = float4_any{v[0], v[1], v[2], v[3]};
+    else if (type == L2_F16) *(anyh *)((_Float16 *)p + i) = anyh{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+    else *(anyb *)((uint16_t *)p + i) = anyb{float_bf16(v[0]), float_bf16(v[1]), float_bf16(v[2]), float_bf16(v[3])};
+}
+
+__device__ __forceinline__ void store8(void *p, int type, int64_t i, const f8 &v) {
+    if (type != L2_F32) {
+        typedef uint16_t any __attribute__((ext_vector_type(8), aligned(2)));
+        any c;
+        for (int j = 0; j < 8; j++) c[j] = type == L2_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v[j]) : float_bf16(v[j]);
+        *(any *)((uint16_t *)p + i) = c;
+    } else {
+        store4(p, type, i, f4{v[0], v[1], v[2], v[3]});
+        store4(p, type, i + 4, f4{v[4], v[5], v[6], v[7]});
+    }
+}
+
 } // namespace kv
 #endif
