@@ -114,15 +114,12 @@ struct Cut {
 
 struct Place {
     int bin, bin1;
-    uint32_t before;
+    u64 before;
 };
 
 struct Shared {
     double exp2[1024];
-    union {
-        u64 mass[kBins];
-        uint32_t light[kBins]; // rounded weights
-    };
+    u64 mass[kBins];
     uint32_t count[kBins];
     u64 part[kWaves];
     struct {
@@ -191,11 +188,12 @@ struct Row {
     // f(j, four logits, id of the first) for this thread's part of each chunk
     template <class F>
     __device__ __forceinline__ void fours(F f) const {
-        Four next = load(0);
+        Four next = load(0), then = load(1);
 #pragma unroll 1
         for (int j = 0; j < chunks(); j++) {
             const Four v = next;
-            if (j + 1 < chunks()) next = load(j + 1);
+            next = then;
+            if (j + 2 < chunks()) then = load(j + 2);
             f(j, v.v, kChunk * j + 4 * (int)threadIdx.x);
         }
     }
@@ -230,11 +228,12 @@ __device__ __forceinline__ V behind_waves(Shared &sh, V upto) {
 }
 
 // The first bins up to which `of` sums to at least `t0` (`t1`), and what is before the first; kBins - 1 if none.
-__device__ __forceinline__ Place first_bins(Shared &sh, const uint32_t *of, uint32_t t0, uint32_t t1) {
+template <class V>
+__device__ __forceinline__ Place first_bins(Shared &sh, const V *of, V t0, V t1) {
     const int tid = threadIdx.x;
-    const uint32_t a = of[2 * tid], b = of[2 * tid + 1];
+    const V a = of[2 * tid], b = of[2 * tid + 1];
     if (tid == 0) sh.place = {kBins - 1, kBins - 1, 0};
-    const uint32_t upto = behind_waves(sh, wave_scan(a + b)), at = upto - b, under = at - a;
+    const V upto = behind_waves(sh, wave_scan(a + b)), at = upto - b, under = at - a;
     if (upto >= t0 && (under < t0 || tid == 0)) sh.place.bin = at >= t0 ? 2 * tid : 2 * tid + 1, sh.place.before = at >= t0 ? under : at; // one thread
     if (upto >= t1 && (under < t1 || tid == 0)) sh.place.bin1 = at >= t1 ? 2 * tid : 2 * tid + 1;
     __syncthreads();
@@ -316,7 +315,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const T *logits, int v
     const int k = s.top_k ? s.top_k[r] : s.top_k0;
     const float p = s.top_p ? s.top_p[r] : s.top_p0, least_p = s.min_p ? s.min_p[r] : s.min_p0, u = s.u ? s.u[r] : s.u0;
     sh.exp2[tid] = kExp2.v[tid];
-    for (int i = tid; i < kBins; i += kThreads) sh.count[i] = 0, sh.light[i] = 0;
+    for (int i = tid; i < kBins; i += kThreads) sh.count[i] = 0, sh.mass[i] = 0;
     if (tid == 0) sh.n = 0;
 
     // the first of the order
@@ -356,7 +355,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const T *logits, int v
         if (k <= kThreads) { // as many tokens as threads whose largest logit lies in a bin or before
             atomicAdd(&sh.count[bins(most)], 1u);
             __syncthreads();
-            last = first_bins(sh, sh.count, k, k).bin;
+            last = first_bins<uint32_t>(sh, sh.count, k, k).bin;
             sh.count[tid] = sh.count[tid + kThreads] = 0;
             __syncthreads();
         }
@@ -368,7 +367,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const T *logits, int v
                     if (bins.place(x[e]) < end) atomicAdd(&sh.count[bins(x[e])], 1u);
         });
         __syncthreads();
-        const Place place = first_bins(sh, sh.count, k, k);
+        const Place place = first_bins<uint32_t>(sh, sh.count, k, k);
         const int bin = place.bin;
         const bool few = sh.count[bin] <= kList && bin < kBins - 1;
         bool found = false;
@@ -392,7 +391,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const T *logits, int v
         __syncthreads();
         if (tid == 0) sh.n = 0;
         if (p < 1.f)
-            for (int i = tid; i < kBins; i += kThreads) sh.light[i] = 0;
+            for (int i = tid; i < kBins; i += kThreads) sh.mass[i] = 0;
         __syncthreads();
     }
     const double least_w = ceil((double)fminf(fmaxf(least_p, 0.f), 1.f) * 0x1p44);
@@ -455,8 +454,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const T *logits, int v
     };
     bool done = false;
     if (p < 1.f) {
-        // weights as whole numbers of 32 bits that sums of all fit, and the sum of all as floats have it
-        const float slope = -1.44269504f / 128.f, unit = __builtin_bit_cast(float, (uint32_t)(127 + __builtin_clz((uint32_t)vocab)) << 23);
+        // weights of fp32 as multiples of 2^-31, and the sum of all as floats have it
+        const float slope = -1.44269504f / 128.f;
         const bool some = cut.id != 0x7FFFFFFF;
         float part = 0.f;
         row.fours([&](int, const float (&x)[4], int id) {
@@ -467,8 +466,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const T *logits, int v
                 float m = __builtin_amdgcn_exp2f(fmaxf(d, 0.f) * slope);
                 if (some) m = cut.has(x[e], id + e) ? m : 0.f;
                 part += m;
-                const uint32_t whole = (uint32_t)fmaf(m, unit, 0.5f);
-                if (whole && d < (float)(kBins - 1)) atomicAdd(&sh.light[(int)d], whole);
+                const uint32_t whole = (uint32_t)(m * 0x1p31f);
+                if (whole && d < (float)(kBins - 1)) atomicAdd(&sh.mass[(int)d], (u64)whole);
             }
         });
         for (int o = 32; o; o >>= 1) part += __shfl_xor(part, o);
@@ -479,8 +478,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const T *logits, int v
 #pragma unroll
         for (int i = 0; i < kWaves; i++) part += parts[i];
         __syncthreads();
-        const float margin = part * 0x1p-13f, near = fmaxf(p, 0.f) * part;
-        const Place in_question = first_bins(sh, sh.light, (uint32_t)(fmaxf(near - margin, 0.f) * unit), (uint32_t)((near + margin) * unit));
+        const float margin = part * 0x1p-16f, near = fmaxf(p, 0.f) * part;
+        const Place in_question = first_bins<u64>(sh, sh.mass, (u64)(fmaxf(near - margin, 0.f) * 0x1p31f), (u64)((near + margin) * 0x1p31f));
         exact(std::true_type{}, (float)in_question.bin, in_question.bin1 == kBins - 1 ? __builtin_inff() : (float)(in_question.bin1 + 1));
         all = block_sum(all), front = block_sum(front);
         const double share = ceil((double)p * (double)all);
