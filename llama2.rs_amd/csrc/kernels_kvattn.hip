@@ -132,6 +132,12 @@ __device__ __forceinline__ u4 finite(u4 v, bool &odd) {
 
 constexpr int kNarrowRows = 16, kNarrowWaves = 4;
 
+// How a launch cuts positions: `splits` parts of `per` tiles each, `stride` parts of a row in the workspace; and the query rows per kv head of a sequence up to which
+// it is the narrow kernel's.
+struct Cut {
+    int splits, per, stride, narrow;
+};
+
 // A query row's part: what a block found of it.  `off` is common to the weights in acc and sum.
 struct Parts {
     float *acc;   // [row][head][split][D]
@@ -142,7 +148,7 @@ struct Parts {
 // four waves tiles of 64 positions (32 of 16-bit cells) in turn, straight from memory into registers: 8 KB of keys and 8 KB of values, the next tile's keys
 // asked for once this one's scores are there and its values once this one's are summed.
 template <int KV, int NP, int D>
-__global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, int splits, int stride, int narrow) {
+__global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, Cut cut) {
     using C = Cells<KV>;
     using Frag = typename C::Frag;
     constexpr int TT = 64 / C::kSize, ST = TT / 16, CH = TT / 4, FR = 2 / C::kSize, KL = D * C::kSize / 64, DT = D / 16, VS = TT / 32;
@@ -150,41 +156,14 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
     const kv::Seq s = kv::sequence(b, i);
     const int group = a.n_heads / l.n_heads, rows = s.rows * group;
-    if (rows == 0 || rows > narrow) return;
+    if (rows == 0 || rows > cut.narrow) return;
     const int base = s.length - s.rows; // position of the first row
     const bool real = m < rows;
     const int pos = real ? base + m / group : -1;
     const int64_t q_row = s.first + (real ? m / group : 0), head = h * group + (real ? m % group : 0);
 
-    // q: this lane's row, the dimensions that lie across from its 16 bytes of a key
-    Frag q[D / 32][NP];
-    float c; // exponent of two per unit of the scores' sums
-    {
-        f8 x[D / 32];
-        float top = 0.f;
-#pragma unroll
-        for (int k = 0; k < D / 32; k++) {
-            const int d = (k / FR) * (64 / C::kSize) + (16 / C::kSize) * g + 8 * (k % FR);
-            x[k] = kv::load8(a.q, a.type, q_row * a.q_stride + head * D + d);
-#pragma unroll
-            for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[k][j]));
-        }
-        c = a.scale * kLog2e;
-        if (C::kHalf) {
-            top = lanes::rows_max(top);
-            const int e = top > 0.f && top < kInf ? 15 - __builtin_amdgcn_frexp_expf(top) : 0; // the largest in [2^14, 2^15)
-#pragma unroll
-            for (int k = 0; k < D / 32; k++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) x[k][j] = ldexpf(x[k][j], e);
-            c = ldexpf(c, -e);
-        }
-#pragma unroll
-        for (int k = 0; k < D / 32; k++) pieces<Frag, typename C::One, NP>(x[k], q[k]);
-    }
-
     const Range range = range_of<TT>(a, base, s.length - 1);
-    const int per = (range.n + splits - 1) / splits, begin = min(split * per, range.n), end = min(begin + per, range.n);
+    const int begin = min(split * cut.per, range.n), end = min(begin + cut.per, range.n);
     const int size = 1 << l.page_shift;
     const char *kb = (const char *)l.k, *vb = (const char *)l.v;
 
@@ -224,16 +203,48 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
         }
     };
 
-    f4 acc[DT] = {};
-    float off = -kInf, sum = 0.f;
+    // What the first tile waits for is asked for in the order of its waits: pages and q, then keys and values.
     int n = begin + w;
+    page_k = page_v = -1;
+    if (n < end) pages(n);
+    kv::raw8 q_raw[D / 32];
+#pragma unroll
+    for (int k = 0; k < D / 32; k++)
+        q_raw[k] = kv::load_raw8(a.q, a.type, q_row * a.q_stride + head * D + (k / FR) * (64 / C::kSize) + (16 / C::kSize) * g + 8 * (k % FR));
+    int here = page_v;
     if (n < end) {
-        pages(n);
         load_k(n, page_k, page_v);
         load_v(n, page_v);
+        if (n + kNarrowWaves < end) pages(n + kNarrowWaves);
     }
-    int here = page_v;
-    if (n + kNarrowWaves < end) pages(n + kNarrowWaves);
+    // q: this lane's row, the dimensions that lie across from its 16 bytes of a key
+    Frag q[D / 32][NP];
+    float c; // exponent of two per unit of the scores' sums
+    {
+        f8 x[D / 32];
+        float top = 0.f;
+#pragma unroll
+        for (int k = 0; k < D / 32; k++) {
+            x[k] = kv::values8(q_raw[k], a.type);
+#pragma unroll
+            for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[k][j]));
+        }
+        c = a.scale * kLog2e;
+        if (C::kHalf) {
+            top = lanes::rows_max(top);
+            const int e = top > 0.f && top < kInf ? 15 - __builtin_amdgcn_frexp_expf(top) : 0; // the largest in [2^14, 2^15)
+#pragma unroll
+            for (int k = 0; k < D / 32; k++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[k][j] = ldexpf(x[k][j], e);
+            c = ldexpf(c, -e);
+        }
+#pragma unroll
+        for (int k = 0; k < D / 32; k++) pieces<Frag, typename C::One, NP>(x[k], q[k]);
+    }
+
+    f4 acc[DT] = {};
+    float off = -kInf, sum = 0.f;
     for (; n < end; n += kNarrowWaves) {
         const int t0 = range.tile(n) * TT;
         const bool more = n + kNarrowWaves < end;
@@ -356,40 +367,63 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
             v += *(const f4 *)&sh_acc[y][r][d] * f;
         }
         const int64_t row = s.first + r / group, hq = h * group + r % group;
-        if (splits == 1) {
+        if (cut.splits == 1) {
             const float inv = total == 0.f ? 0.f : 1.f / total;
             for (int j = 0; j < 4; j++) v[j] = total == 0.f ? 0.f : v[j] * inv;
             kv::store4(a.out, a.type, row * a.out_stride + hq * D + d, v);
         } else {
-            const int64_t at = (row * a.n_heads + hq) * stride + split;
+            const int64_t at = (row * a.n_heads + hq) * cut.stride + split;
             *(f4 *)(parts.acc + at * D + d) = v;
             if (d == 0) parts.stat[at] = make_float2(o, total);
         }
     }
 }
 
-// Joins the parts of each query row: one wave per row and head.  NARROW: block x has row x % most of sequence x / most, most rows at the most; else row x.
+__device__ __forceinline__ float wave_max(float v) {
+    v = lanes::rows_max(v);
+    for (int o = 8; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+
+// Joins the parts of each query row: a block per row and head, its waves parts in turn.  NARROW: block x has row x % most of sequence x / most, most rows at the most;
+// else row x.
+constexpr int kJoinWaves = 4;
 template <int D, bool NARROW>
-__global__ __launch_bounds__(64) void kv_join_kernel(l2_kvbatch b, KvAttention a, Parts parts, int splits, int stride, int group, int most) {
-    const int hq = blockIdx.y, lane = threadIdx.x;
+__global__ __launch_bounds__(64 * kJoinWaves) void kv_join_kernel(l2_kvbatch b, KvAttention a, Parts parts, int splits, int stride, int group, int most) {
+    const int hq = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int i = NARROW ? (int)blockIdx.x / most : kv::sequence_of(b, blockIdx.x);
     if (i >= b.n_seqs) return;
     const kv::Seq s = kv::sequence(b, i);
     const int row = NARROW ? s.first + (int)blockIdx.x % most : blockIdx.x;
-    if (row - s.first >= s.rows || ((int64_t)s.rows * group <= most * group) != NARROW) return;
+    if (row - s.first >= s.rows || (s.rows <= most) != NARROW) return;
     const int64_t at = ((int64_t)row * a.n_heads + hq) * stride;
-    float o = -kInf, total = 0.f;
-    for (int x = 0; x < splits; x++) o = fmaxf(o, parts.stat[at + x].x);
+    __shared__ float sh_acc[kJoinWaves][D], sh_sum[kJoinWaves];
+    float o = -kInf;
+    for (int x = lane; x < splits; x += 64) o = fmaxf(o, parts.stat[at + x].x);
+    o = wave_max(o);
     constexpr int E = D / 64;
-    float v[E] = {};
-    for (int x = 0; x < splits; x++) {
+    float v[E] = {}, total = 0.f;
+#pragma unroll 4
+    for (int x = w; x < splits; x += kJoinWaves) {
         const float2 st = parts.stat[at + x];
-        if (st.y == 0.f && st.x == -kInf) continue;
-        const float f = st.x == o ? 1.f : __builtin_amdgcn_exp2f(st.x - o);
-        total += st.y * f;
-        for (int e = 0; e < E; e++) v[e] += parts.acc[(at + x) * D + E * lane + e] * f;
+        float part[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) part[e] = parts.acc[(at + x) * D + E * lane + e];
+        const bool none = st.y == 0.f && st.x == -kInf; // nothing of it is there
+        const float f = none ? 0.f : st.x == o ? 1.f : __builtin_amdgcn_exp2f(st.x - o);
+        total += none ? 0.f : st.y * f;
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] += none ? 0.f : part[e] * f;
     }
-    for (int e = 0; e < E; e++) kv::store(a.out, a.type, row * a.out_stride + (int64_t)hq * D + E * lane + e, total == 0.f ? 0.f : v[e] / total);
+#pragma unroll
+    for (int e = 0; e < E; e++) sh_acc[w][E * lane + e] = v[e];
+    if (lane == 0) sh_sum[w] = total;
+    __syncthreads();
+    if (threadIdx.x >= D) return;
+    float sum = 0.f, acc = 0.f;
+#pragma unroll
+    for (int x = 0; x < kJoinWaves; x++) sum += sh_sum[x], acc += sh_acc[x][threadIdx.x];
+    kv::store(a.out, a.type, row * a.out_stride + (int64_t)hq * D + threadIdx.x, sum == 0.f ? 0.f : acc / sum);
 }
 
 typedef float f16v __attribute__((ext_vector_type(16)));
@@ -402,12 +436,6 @@ constexpr int kWideWaves = 4, kWideRows = 32 * kWideWaves, kWideThreads = 64 * k
 template <int PER_ROW>
 __device__ __forceinline__ int piece_at(int r, int x) {
     return r * PER_ROW + (PER_ROW == 16 ? x ^ (r & 15) : x ^ (r >> 1 & 7));
-}
-
-__device__ __forceinline__ float wave_max(float v) {
-    v = lanes::rows_max(v);
-    for (int o = 8; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
 }
 
 // Values that are the same in every lane, in scalar registers.
@@ -433,7 +461,7 @@ __device__ __forceinline__ void wait_lds_loads() { asm volatile("s_waitcnt vmcnt
 // bits, the next tile on its way meanwhile: codes of 8 bits into registers, to be converted once for all four waves, 16-bit cells straight into LDS.  A tile is
 // four runs of 16 positions, each in one page; their addresses are computed once per wave.
 template <int KV, int NP, int D>
-__global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, int splits, int stride, int narrow) {
+__global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, Cut cut) {
     using C = Cells<KV>;
     using Frag = typename C::Frag;
     constexpr int TT = 64, PK = D / 8, DT = D / 32, KS = D / 16, LOADS = TT * D * C::kSize / 16 / kWideThreads;
@@ -445,18 +473,18 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
     __shared__ int sh_seq, sh_tile;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, hh = lane >> 5;
     const int group = a.n_heads / l.n_heads;
-    const int h = __builtin_amdgcn_readfirstlane(blockIdx.x % l.n_heads), split = __builtin_amdgcn_readfirstlane(blockIdx.x / l.n_heads % splits);
+    const int h = __builtin_amdgcn_readfirstlane(blockIdx.x % l.n_heads), split = __builtin_amdgcn_readfirstlane(blockIdx.x / l.n_heads % cut.splits);
 
     // which sequence's rows: the tiles of all sequences one behind the other
     {
-        int at = blockIdx.x / (l.n_heads * splits);
+        int at = blockIdx.x / (l.n_heads * cut.splits);
         if (tid == 0) sh_seq = -1;
         __syncthreads();
         for (int i0 = 0; i0 < b.n_seqs; i0 += 64) {
             int tiles = 0;
             if (i0 + lane < b.n_seqs) {
                 const int64_t r = (int64_t)kv::sequence(b, i0 + lane).rows * group;
-                tiles = r > narrow ? (int)((r + kWideRows - 1) / kWideRows) : 0;
+                tiles = r > cut.narrow ? (int)((r + kWideRows - 1) / kWideRows) : 0;
             }
             int upto = tiles;
             for (int o = 1; o < 64; o <<= 1) {
@@ -485,14 +513,18 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
     const int b_last = __builtin_amdgcn_readfirstlane(base + (min((tile + 1) * kWideRows, rows) - 1) / group);
 
     Frag q[KS][NP];
-    float c;
+    float c = a.scale * kLog2e;
     {
+        kv::raw8 raw[KS];
+#pragma unroll
+        for (int k = 0; k < KS; k++) raw[k] = kv::load_raw8(a.q, a.type, q_row * a.q_stride + head * D + 16 * k + 8 * hh);
         float top = 0.f;
-        c = a.scale * kLog2e;
         int e = 0;
         if (C::kHalf) {
+#pragma unroll
             for (int k = 0; k < KS; k++) {
-                const f8 x = kv::load8(a.q, a.type, q_row * a.q_stride + head * D + 16 * k + 8 * hh);
+                const f8 x = kv::values8(raw[k], a.type);
+#pragma unroll
                 for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[j]));
             }
             const lanes::Both t = lanes::both32(top);
@@ -502,15 +534,16 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
         }
 #pragma unroll
         for (int k = 0; k < KS; k++) {
-            f8 x = kv::load8(a.q, a.type, q_row * a.q_stride + head * D + 16 * k + 8 * hh);
+            f8 x = kv::values8(raw[k], a.type);
             if (C::kHalf)
+#pragma unroll
                 for (int j = 0; j < 8; j++) x[j] = ldexpf(x[j], e);
             pieces<Frag, typename C::One, NP>(x, q[k]);
         }
     }
 
     const Range range = range_of<TT>(a, b_first, b_last);
-    const int per = __builtin_amdgcn_readfirstlane((range.n + splits - 1) / splits), begin = min(split * per, range.n), end = min(begin + per, range.n);
+    const int begin = min(split * cut.per, range.n), end = min(begin + cut.per, range.n);
     const int size = 1 << l.page_shift;
 
     struct Pages {
@@ -730,7 +763,7 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
     const lanes::Both s2 = lanes::both32(sum);
     sum = s2.lo + s2.hi;
     if (!real) return;
-    if (splits == 1) {
+    if (cut.splits == 1) {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
         for (int y = 0; y < DT; y++)
@@ -743,7 +776,7 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
                 kv::store4(a.out, a.type, at, v);
             }
     } else {
-        const int64_t at = (q_row * a.n_heads + head) * stride + split;
+        const int64_t at = (q_row * a.n_heads + head) * cut.stride + split;
 #pragma unroll
         for (int y = 0; y < DT; y++)
 #pragma unroll
@@ -753,7 +786,7 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
     }
 }
 
-typedef void (*AttnKernel)(KvLayer, l2_kvbatch, KvAttention, Parts, int, int, int);
+typedef void (*AttnKernel)(KvLayer, l2_kvbatch, KvAttention, Parts, Cut);
 #define SIZES(kernel, kv, np) {kernel<kv, np, 64>, kernel<kv, np, 128>}
 #define ALL(kernel)                                                                                                                             \
     {{SIZES(kernel, 0, 1), SIZES(kernel, 0, 2), {}}, {SIZES(kernel, 1, 1), SIZES(kernel, 1, 2), {}}, {SIZES(kernel, 2, 1), SIZES(kernel, 2, 2), {}}, \
@@ -778,22 +811,28 @@ void kv_attention_plan(const KvLayer &l, int kv_type, const l2_kvbatch &b, const
         if (a.window) seen = std::min<int64_t>(seen, (int64_t)a.window + std::min(rows, per_tile) + a.sinks + 2 * tt);
         return (seen + tt - 1) / tt;
     };
-    auto parts_of = [&](int64_t blocks, int64_t full, int64_t tiles, int64_t least) {
-        return (int)std::max<int64_t>(1, std::min<int64_t>((full + blocks - 1) / blocks, tiles / least));
+    // parts so that `full` blocks come to be, of `least` tiles or more
+    auto parts_of = [&](int64_t blocks, int64_t full, int64_t tiles, int64_t least, int *splits, int *per) {
+        const int64_t parts = std::max<int64_t>(1, std::min<int64_t>((full + blocks - 1) / blocks, tiles / least));
+        *per = (int)((tiles + parts - 1) / parts);
+        *splits = *per ? (int)((tiles + *per - 1) / *per) : 1;
     };
     plan->wide = rows * group > kNarrowRows;
     // A single sequence is the one kernel's or the other's; several may be some of each.
     plan->narrow_rows = group > kNarrowRows || (plan->wide && seqs == 1) ? 0 : kNarrowRows / group * group;
     plan->narrow_splits = plan->wide_splits = 1;
+    const char *e1 = getenv("KVA"), *e2 = getenv("KVB");
     if (plan->narrow_rows)
-        plan->narrow_splits = parts_of(seqs * l.n_heads, 2 * cu_count(), tiles_seen(kv_type <= L2_KV_E4M3 ? 64 : 32, kNarrowRows), 2 * kNarrowWaves);
+        parts_of(seqs * l.n_heads, (e1 ? atoi(e1) : 2) * cu_count(), tiles_seen(kv_type <= L2_KV_E4M3 ? 64 : 32, kNarrowRows), (e2 ? atoi(e2) : 2) * kNarrowWaves, &plan->narrow_splits,
+                 &plan->narrow_per);
     // row tiles of all sequences, at most: their whole ones, and a last one of each that has more rows than the narrow kernel takes
     const int64_t all = (int64_t)b.n_rows * group;
     plan->wide_tiles = (int)std::min<int64_t>(all / kWideRows + std::min<int64_t>(seqs, all / (plan->narrow_rows + 1)), 1 << 26);
     // blocks for every CU's room: two, or one of those with more registers
     const int room = pieces_index(kv_type, a.type) == 0 ? 2 : 1;
     if (plan->wide)
-        plan->wide_splits = parts_of(std::max<int64_t>(all / kWideRows, 1) * l.n_heads, room * cu_count(), tiles_seen(64, (kWideRows + group - 1) / group), 4);
+        parts_of(std::max<int64_t>(all / kWideRows, 1) * l.n_heads, room * cu_count(), tiles_seen(64, (kWideRows + group - 1) / group), 4, &plan->wide_splits,
+                 &plan->wide_per);
     plan->stride = std::max(plan->narrow_splits, plan->wide_splits);
     plan->workspace = plan->stride > 1 ? (size_t)b.n_rows * a.n_heads * plan->stride * (l.head_size * 4 + 8) : 0;
 }
@@ -806,18 +845,18 @@ int kv_attention_launch(const KvLayer &l, int kv_type, const l2_kvbatch &b, cons
     if (plan.wide && plan.wide_tiles) {
         const int64_t blocks = (int64_t)plan.wide_tiles * l.n_heads * plan.wide_splits;
         if (blocks >= (int64_t)1 << 31) return l2_fail(L2_ERR_RANGE, "%d rows of %d heads", b.n_rows, a.n_heads);
-        l2_launch(kWide[kv_type][np][big], dim3((unsigned)blocks), dim3(kWideThreads), 0, st, l, b, a, parts, plan.wide_splits, plan.stride,
-                  plan.narrow_rows);
+        l2_launch(kWide[kv_type][np][big], dim3((unsigned)blocks), dim3(kWideThreads), 0, st, l, b, a, parts,
+                  Cut{plan.wide_splits, plan.wide_per, plan.stride, plan.narrow_rows});
     }
     if (plan.narrow_rows)
-        l2_launch(kNarrow[kv_type][np][big], dim3(plan.narrow_splits, l.n_heads, b.n_seqs), dim3(64 * kNarrowWaves), 0, st, l, b, a, parts, plan.narrow_splits,
-                  plan.stride, plan.narrow_rows);
+        l2_launch(kNarrow[kv_type][np][big], dim3(plan.narrow_splits, l.n_heads, b.n_seqs), dim3(64 * kNarrowWaves), 0, st, l, b, a, parts,
+                  Cut{plan.narrow_splits, plan.narrow_per, plan.stride, plan.narrow_rows});
     const int most = plan.narrow_rows / group; // rows of a sequence that the narrow kernel takes
     if (plan.narrow_rows && plan.narrow_splits > 1)
-        l2_launch(kJoin[big][1], dim3(b.n_seqs * std::min(most, b.max_rows), a.n_heads), dim3(64), 0, st, b, a, parts, plan.narrow_splits, plan.stride, group,
+        l2_launch(kJoin[big][1], dim3(b.n_seqs * std::min(most, b.max_rows), a.n_heads), dim3(64 * kJoinWaves), 0, st, b, a, parts, plan.narrow_splits, plan.stride, group,
                   std::min(most, b.max_rows));
     if (plan.wide && plan.wide_splits > 1)
-        l2_launch(kJoin[big][0], dim3(b.n_rows, a.n_heads), dim3(64), 0, st, b, a, parts, plan.wide_splits, plan.stride, group, most);
+        l2_launch(kJoin[big][0], dim3(b.n_rows, a.n_heads), dim3(64 * kJoinWaves), 0, st, b, a, parts, plan.wide_splits, plan.stride, group, most);
     L2_HIP(hipGetLastError());
     return L2_OK;
 }

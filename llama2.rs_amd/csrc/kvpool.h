@@ -39,7 +39,8 @@ struct KvAttnPlan {
     size_t workspace;               // bytes
     bool wide;                      // whether there may be sequences of more rows than ..
     int narrow_rows;                // .. the narrow kernel takes, per kv head; 0: it takes none
-    int narrow_splits, wide_splits; // parts that positions are cut into
+    int narrow_splits, wide_splits; // parts that positions are cut into,
+    int narrow_per, wide_per;       // each of so many tiles
     int stride;                     // the larger of both: parts of a row in the workspace
     int wide_tiles;                 // tiles of rows of the wide kernel, at most
 };
@@ -102,24 +103,32 @@ __device__ __forceinline__ void store(void *p, int type, int64_t i, float v) {
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f8 __attribute__((ext_vector_type(8)));
 
-// Eight values of a row of the caller's, aligned as their type is.
-__device__ __forceinline__ f8 load8(const void *p, int type, int64_t i) {
-    typedef float any __attribute__((ext_vector_type(8), aligned(4)));
-    typedef _Float16 anyh __attribute__((ext_vector_type(8), aligned(2)));
-    typedef uint16_t anyb __attribute__((ext_vector_type(8), aligned(2)));
+// Eight values of a row of the caller's, aligned as their type is; as they lie in memory first, so that several are on their way at once.
+typedef uint32_t raw8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ raw8 load_raw8(const void *p, int type, int64_t i) {
+    typedef uint32_t any8 __attribute__((ext_vector_type(8), aligned(4)));
+    typedef uint32_t any4 __attribute__((ext_vector_type(4), aligned(2)));
+    if (type == L2_F32) {
+        const any8 v = *(const any8 *)((const float *)p + i);
+        return raw8{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+    }
+    const any4 v = *(const any4 *)((const uint16_t *)p + i);
+    return raw8{v[0], v[1], v[2], v[3], 0, 0, 0, 0};
+}
+__device__ __forceinline__ f8 values8(const raw8 &v, int type) {
     f8 x;
     if (type == L2_F32) {
-        const any v = *(const any *)((const float *)p + i);
-        for (int j = 0; j < 8; j++) x[j] = v[j];
+        x = __builtin_bit_cast(f8, v);
     } else if (type == L2_F16) {
-        const anyh v = *(const anyh *)((const _Float16 *)p + i);
-        for (int j = 0; j < 8; j++) x[j] = (float)v[j];
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = (float)__builtin_bit_cast(_Float16, (uint16_t)(v[j / 2] >> 16 * (j % 2)));
     } else {
-        const anyb v = *(const anyb *)((const uint16_t *)p + i);
-        for (int j = 0; j < 8; j++) x[j] = bf16_float(v[j]);
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = bf16_float((uint16_t)(v[j / 2] >> 16 * (j % 2)));
     }
     return x;
 }
+__device__ __forceinline__ f8 load8(const void *p, int type, int64_t i) { return values8(load_raw8(p, type, i), type); }
 
 __device__ __forceinline__ void store4(void *p, int type, int64_t i, const f4 &v) {
     typedef _Float16 anyh __attribute__((ext_vector_type(4), aligned(2)));
