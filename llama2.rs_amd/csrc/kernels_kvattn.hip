@@ -113,9 +113,12 @@ __device__ __forceinline__ Range range_of(const KvAttention &a, int pos_first, i
     return {se, from, se + end - from};
 }
 
-__device__ __forceinline__ bool visible(const KvAttention &a, int t, int pos) {
-    return t <= pos && (!a.window || t > pos - a.window || t < a.sinks);
-}
+// What the row of position pos sees: up to pos, from `from` on or below `sinks`.
+struct Seen {
+    int pos, from, sinks;
+    __device__ __forceinline__ Seen(const KvAttention &a, int pos) : pos(pos), from(a.window ? max(pos - a.window + 1, 0) : 0), sinks(a.sinks) {}
+    __device__ __forceinline__ bool operator()(int t) const { return (t <= pos) & ((t >= from) | (t < sinks)); }
+};
 
 // v with fp16 (bf16) numbers that are not finite as zeros, and whether there are any.
 template <int KV>
@@ -159,7 +162,7 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
     if (rows == 0 || rows > cut.narrow) return;
     const int base = s.length - s.rows; // position of the first row
     const bool real = m < rows;
-    const int pos = real ? base + m / group : -1;
+    const Seen seen(a, real ? base + m / group : -1);
     const int64_t q_row = s.first + (real ? m / group : 0), head = h * group + (real ? m % group : 0);
 
     const Range range = range_of<TT>(a, base, s.length - 1);
@@ -271,7 +274,7 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
             for (int x = 0; x < ST; x++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const bool see = here >= 0 && visible(a, t0 + CH * g + 4 * x + r, pos);
+                    const bool see = (here >= 0) & seen(t0 + CH * g + 4 * x + r);
                     sc[x][r] = see ? sc[x][r] : -kInf;
                     if (C::kEight) vs[x][r] = see ? vs[x][r] : 0.f;
                 }
@@ -322,7 +325,7 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
 #pragma unroll 1
             for (int y = 0; y < TT; y++) {
                 const int t = t0 + y, page = kv::page_at(b, l.n_pages, i, t >> l.page_shift);
-                if (page < 0 || !visible(a, t, pos)) continue;
+                if (page < 0 || !seen(t)) continue;
                 int first = 4 * g; // unknown, so that the places are not worked out ahead of the loop
                 asm volatile("" : "+v"(first));
                 const uint16_t *p = (const uint16_t *)vb + (((int64_t)page * l.n_heads + h) * D * size + (t & (size - 1)));
@@ -430,7 +433,7 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ f16v mfma32(const h8 &a, const h8 &b, const f16v &c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f16v mfma32(const b8 &a, const b8 &b, const f16v &c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
-constexpr int kWideWaves = 4, kWideRows = 32 * kWideWaves, kWideThreads = 64 * kWideWaves;
+constexpr int kWideWaves = 8, kWideRows = 32 * kWideWaves, kWideThreads = 64 * kWideWaves;
 
 // Where 16-byte piece x of row r lies in a tile of rows of 128 (256) bytes: the sixteen rows that a 16-byte LDS read takes together then meet sixteen places.
 template <int PER_ROW>
@@ -457,20 +460,29 @@ __device__ __forceinline__ void lds_load(uint32_t lds, const char *at) {
 }
 __device__ __forceinline__ void wait_lds_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// Longer chunks.  A block has 128 query rows of one sequence and kv head, a wave 32 of them; keys and values come in tiles of 64 positions through LDS, in 16
-// bits, the next tile on its way meanwhile: codes of 8 bits into registers, to be converted once for all four waves, 16-bit cells straight into LDS.  A tile is
-// four runs of 16 positions, each in one page; their addresses are computed once per wave.
+// A barrier that waits for this wave's LDS accesses and for no loads from memory.
+__device__ __forceinline__ void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Longer chunks.  A block has 256 query rows of one sequence and kv head, a wave 32 of them; keys and values come in tiles of 64 positions through LDS, in 16
+// bits, the next one or two on their way meanwhile: codes of 8 bits into registers, to be converted once for all waves, 16-bit cells straight into LDS.  A tile is four
+// runs of 16 positions, each in one page; their addresses are computed once per wave.
+//
+// The two waves of a SIMD take turns: while the first four waves have the matrix cores (the weighted sum of the tile before, then the scores of this one), the
+// last four have the vector ALUs (exponentials, the next tile's conversion), half a tile behind, and the barriers between keep it so.  Left to themselves, waves of
+// two blocks had either unit busy for 28 and 52 % of the time, hardly ever together.  In steps of half a tile, 0 the first: the first four do the products of tile i in step 2 i
+// and its exponentials in 2 i + 1, the others each a step later.  So keys of tile i are read in steps 2 i and 2 i + 1, its values in 2 i + 2 and 2 i + 3, its scales in 2 i + 1 and 2 i + 2;
+// with two places for keys and three for the rest, tile i + 1 may be written from step 2 i on, and is there before 2 i + 2.
 template <int KV, int NP, int D>
-__global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, Cut cut) {
+__global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, Cut cut) {
     using C = Cells<KV>;
     using Frag = typename C::Frag;
-    constexpr int TT = 64, PK = D / 8, DT = D / 32, KS = D / 16, LOADS = TT * D * C::kSize / 16 / kWideThreads;
+    constexpr int TT = 64, PK = D / 8, DT = D / 32, KS = D / 16, PIECES = TT * D * C::kSize / 16, LOADS = (PIECES + kWideThreads - 1) / kWideThreads;
     constexpr int RUN = 16 * D * C::kSize;        // bytes of 16 rows of K
     constexpr int COL16 = TT * C::kSize / 16;     // 16-byte pieces of the tile's part of a row of V
-    __shared__ __align__(16) u4 sh_k[2][TT * PK], sh_v[2][D * 8];
-    __shared__ __align__(16) float sh_ks[2][TT], sh_vs[2][TT];
-    __shared__ float sh_top[2];
-    __shared__ int sh_seq, sh_tile;
+    __shared__ __align__(16) u4 sh_k[2][TT * PK], sh_v[3][D * 8];
+    __shared__ __align__(16) float sh_ks[3][TT], sh_vs[3][TT];
+    __shared__ float sh_top[3];
+    __shared__ int sh_seq, sh_tile, sh_odd[3];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, hh = lane >> 5;
     const int group = a.n_heads / l.n_heads;
     const int h = __builtin_amdgcn_readfirstlane(blockIdx.x % l.n_heads), split = __builtin_amdgcn_readfirstlane(blockIdx.x / l.n_heads % cut.splits);
@@ -479,6 +491,7 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
     {
         int at = blockIdx.x / (l.n_heads * cut.splits);
         if (tid == 0) sh_seq = -1;
+        if (tid < 3) sh_odd[tid] = -1;
         __syncthreads();
         for (int i0 = 0; i0 < b.n_seqs; i0 += 64) {
             int tiles = 0;
@@ -504,7 +517,7 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
     const int rows = s.rows * group, row0 = tile * kWideRows + 32 * w, base = s.length - s.rows;
     const bool real = row0 + n < rows;
     const int tok = real ? (row0 + n) / group : 0;
-    const int pos = real ? base + tok : -1;
+    const Seen seen(a, real ? base + tok : -1);
     const int64_t q_row = s.first + tok, head = h * group + (real ? (row0 + n) % group : 0);
     // the positions of the wave's rows and of the block's
     const int w_first = __builtin_amdgcn_readfirstlane(base + min(row0, rows - 1) / group);
@@ -546,19 +559,6 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
     const int begin = min(split * cut.per, range.n), end = min(begin + cut.per, range.n);
     const int size = 1 << l.page_shift;
 
-    struct Pages {
-        int p[4];
-    };
-    auto pages = [&](int x) { // of the runs of a tile; what lies behind the table is behind every position too
-        Pages g;
-#pragma unroll
-        for (int y = 0; y < 4; y++) {
-            const int at = min((range.tile(x) * TT + 16 * y) >> l.page_shift, b.max_pages - 1);
-            const int page = uniform_load(b.pages + ((int64_t)i * b.max_pages + at));
-            g.p[y] = (uint32_t)page < (uint32_t)l.n_pages ? page : -1;
-        }
-        return g;
-    };
     // Offsets of this thread's pieces: of K from its run's first byte, of V from the run's first position.  16-bit cells: of the piece whose place in LDS
     // is the thread's.
     constexpr int KX = 1024 / (16 * PK);                    // rows of K in a wave's 1024 bytes of LDS
@@ -567,198 +567,252 @@ __global__ __launch_bounds__(kWideThreads, NP == 1 ? 2 : 1) void kv_wide_kernel(
     const uint32_t k_off = C::kEight ? tid * 16 % RUN : ((k_row & 15) * D + 8 * (lane % PK ^ (PK == 16 ? k_row & 15 : k_row >> 1 & 7))) * 2;
     const int v_run = C::kEight ? v_x : v_x >> 1;
     const uint32_t v_off = (uint32_t)(v_row * size + (C::kEight ? 0 : 8 * (v_x & 1))) * C::kSize, v_step = (uint32_t)(kWideThreads / COL16) * size * C::kSize;
-
     const uint32_t lds_k = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u4 *)&sh_k[0][0] + w * 1024;
     const uint32_t lds_v = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u4 *)&sh_v[0][0] + w * 1024;
+    const bool late = w >= kWideWaves / 2; // of the last four waves
+    const bool loads = PIECES >= kWideThreads || w < PIECES / 64;
+
+    // Whether every row of those from position `first` to `last` sees all of a tile whose pages are there.
+    auto all_visible = [&](int t0, int first, int last) { return t0 + TT - 1 <= first && (!a.window || t0 > last - a.window || t0 + TT <= a.sinks); };
+
     u4 kr[LOADS], vr[LOADS];
     float scale = 0.f;
-    auto load = [&](int x, const Pages &g, int buf) {
+    // Entries of the table for the tile that is asked for next: of the runs of this wave's pieces of K, and of this lane's piece of V.  What lies behind the table is
+    // behind every position too.
+    int k_page[LOADS], v_page = -1;
+    const int32_t *table = b.pages + (int64_t)i * b.max_pages;
+    auto ask_pages = [&](int x) {
         const int t0 = range.tile(x) * TT;
-        const char *kp[4], *vp[4];
-        int64_t ph[4];
 #pragma unroll
-        for (int y = 0; y < 4; y++) {
-            ph[y] = ((int64_t)max(g.p[y], 0) * l.n_heads + h) * size;
-            const int slot = (t0 + 16 * y) & (size - 1);
-            kp[y] = (const char *)l.k + (ph[y] + slot) * D * C::kSize;
-            vp[y] = (const char *)l.v + (ph[y] * D + slot) * C::kSize;
-        }
-        const char *v_at;
-        if (size >= TT) v_at = vp[0] + 16 * C::kSize * v_run;
-        else v_at = v_run < 2 ? (v_run ? vp[1] : vp[0]) : (v_run == 2 ? vp[2] : vp[3]);
-        v_at += v_off;
-#pragma unroll
-        for (int y = 0; y < LOADS; y++) {
-            const int run = (w * 1024 + y * 16 * kWideThreads) / RUN;
-            const char *kb = run < 2 ? (run ? kp[1] : kp[0]) : (run == 2 ? kp[2] : kp[3]);
-            if constexpr (C::kEight) kr[y] = *(const u4 *)(kb + k_off);
-            else lds_load(lds_k + (buf * TT * PK + y * kWideThreads) * 16, kb, k_off);
-        }
-#pragma unroll
-        for (int y = 0; y < LOADS; y++) {
-            if constexpr (C::kEight) vr[y] = *(const u4 *)(v_at + y * v_step);
-            else lds_load(lds_v + (buf * D * 8 + y * kWideThreads) * 16, v_at + y * v_step);
-        }
-        if (C::kEight && w < 2) {
-            const int run = lane >> 4;
-            const int64_t at = run < 2 ? (run ? ph[1] : ph[0]) : (run == 2 ? ph[2] : ph[3]);
-            scale = (w ? l.v_scale : l.k_scale)[at + ((t0 + lane) & (size - 1))];
-        }
+        for (int y = 0; y < LOADS; y++) k_page[y] = uniform_load(table + min((t0 + (w * 1024 + y * 16 * kWideThreads) / RUN * 16) >> l.page_shift, b.max_pages - 1));
+        v_page = table[min((t0 + 16 * v_run) >> l.page_shift, b.max_pages - 1)];
     };
-    auto stage = [&](int buf) {
-        if constexpr (C::kEight) {
+    const int64_t page_cells = (int64_t)l.n_heads * size * D * C::kSize; // bytes of a page's K (V)
+    const char *k_from = (const char *)l.k + (int64_t)h * size * D * C::kSize, *v_from = (const char *)l.v + (int64_t)h * size * D * C::kSize + v_off;
+    int ahead = 0; // which runs have a page: four bits for this tile, then for those behind it that have been asked for
+    // Asks for the tile `by` tiles behind tile x, whose pages have been asked for, and for the pages of the one behind that.
+    auto ask = [&](int x, int by) {
+        x += by;
+        if (x >= end) return;
+        const bool is = (uint32_t)v_page < (uint32_t)l.n_pages;
+        int runs = 15;
+        if (__ballot(!is))
+            for (int y = 0; y < 4; y++) runs &= __ballot(!is && v_run == y) ? ~(1 << y) : 15;
+        ahead |= runs << 4 * by;
+        const int t0 = range.tile(x) * TT, kb = (x - begin) & 1, vb = (x - begin) % 3;
+        if (loads) {
+            const char *v_at = v_from + (int64_t)(is ? v_page : 0) * page_cells + ((t0 + 16 * v_run) & (size - 1)) * C::kSize;
 #pragma unroll
             for (int y = 0; y < LOADS; y++) {
-                const int p = tid + kWideThreads * y, kr_row = p * 16 / (D * C::kSize), kr_x = p % (D * C::kSize / 16), row = v_row + kWideThreads / COL16 * y;
-                sh_k[buf][piece_at<PK>(kr_row, 2 * kr_x)] = __builtin_bit_cast(u4, C::frag(kr[y], 0));
-                sh_k[buf][piece_at<PK>(kr_row, 2 * kr_x + 1)] = __builtin_bit_cast(u4, C::frag(kr[y], 1));
-                sh_v[buf][piece_at<8>(row, 2 * v_x)] = __builtin_bit_cast(u4, C::frag(vr[y], 0));
-                sh_v[buf][piece_at<8>(row, 2 * v_x + 1)] = __builtin_bit_cast(u4, C::frag(vr[y], 1));
+                const int page = (uint32_t)k_page[y] < (uint32_t)l.n_pages ? k_page[y] : 0, run = (w * 1024 + y * 16 * kWideThreads) / RUN;
+                const char *at = k_from + (int64_t)page * page_cells + ((t0 + 16 * run) & (size - 1)) * (D * C::kSize);
+                if constexpr (C::kEight) kr[y] = *(const u4 *)(at + k_off);
+                else lds_load(lds_k + (kb * TT * PK + y * kWideThreads) * 16, at, k_off);
             }
-            if (w < 2) (w ? sh_vs : sh_ks)[buf][lane] = scale;
-            if (w == 1) {
-                const float most = wave_max(scale);
-                if (lane == 0) sh_top[buf] = most;
+#pragma unroll
+            for (int y = 0; y < LOADS; y++) {
+                if constexpr (C::kEight) vr[y] = *(const u4 *)(v_at + y * v_step);
+                else lds_load(lds_v + (vb * D * 8 + y * kWideThreads) * 16, v_at + y * v_step);
             }
-        } else {
+            if (C::kEight && w < 2) { // lane y has run y of V
+                const int page = __shfl(is ? v_page : 0, lane >> 4);
+                scale = (w ? l.v_scale : l.k_scale)[((int64_t)page * l.n_heads + h) * size + ((t0 + lane) & (size - 1))];
+            }
+        }
+        if (x + 1 < end) ask_pages(x + 1);
+    };
+    // Writes the tile `by` tiles behind x, asked for before, to LDS.  16-bit cells are there already: where a row may not see all of the tile, values that are not finite
+    // are taken out (and added to the rows that do see them, one by one).
+    auto put = [&](int x, int by) {
+        x += by;
+        if (x >= end || !loads) return;
+        const int kb = (x - begin) & 1, vb = (x - begin) % 3;
+        if constexpr (!C::kEight) {
             wait_lds_loads();
+            if ((ahead >> 4 * by & 15) == 15 && all_visible(range.tile(x) * TT, b_first, b_last)) return;
+#pragma unroll
+            for (int y = 0; y < LOADS; y++) {
+                bool odd = false;
+                u4 *at = &sh_v[vb][tid + kWideThreads * y];
+                const u4 v = finite<KV>(*at, odd);
+                if (odd) *at = v, sh_odd[vb] = x;
+            }
+            return;
+        }
+#pragma unroll
+        for (int y = 0; y < LOADS; y++) {
+            const int p = tid + kWideThreads * y, kr_row = p * 16 / (D * C::kSize), kr_x = p % (D * C::kSize / 16), row = v_row + kWideThreads / COL16 * y;
+            sh_k[kb][piece_at<PK>(kr_row, 2 * kr_x)] = __builtin_bit_cast(u4, C::frag(kr[y], 0));
+            sh_k[kb][piece_at<PK>(kr_row, 2 * kr_x + 1)] = __builtin_bit_cast(u4, C::frag(kr[y], 1));
+            sh_v[vb][piece_at<8>(row, 2 * v_x)] = __builtin_bit_cast(u4, C::frag(vr[y], 0));
+            sh_v[vb][piece_at<8>(row, 2 * v_x + 1)] = __builtin_bit_cast(u4, C::frag(vr[y], 1));
+        }
+        if (w < 2) (w ? sh_vs : sh_ks)[vb][lane] = scale;
+        if (w == 1) {
+            const float most = wave_max(scale);
+            if (lane == 0) sh_top[vb] = most;
         }
     };
-    // Whether every row of the wave sees all of a tile whose pages are there.
-    auto all_visible = [&](int t0) { return t0 + TT - 1 <= w_first && (!a.window || t0 > w_last - a.window || t0 + TT <= a.sinks); };
 
-    f16v acc[DT] = {};
+    const int kr_row = (n & 0x13) | (n & 4) << 1 | (n & 8) >> 1;
+    // (2 k + hh) ^ x is (hh ^ x) ^ 2 k: a piece's address is the first one's but for the bits of k
+    const uint32_t k_base = 16 * piece_at<PK>(kr_row, hh), v_base = 16 * piece_at<8>(n, hh);
+    auto k_at = [&](int buf, int k, int y) { return *(const u4 *)((const char *)&sh_k[buf][32 * y * PK] + (k_base ^ (32 * k))); };
+    auto v_at = [&](int buf, int y, int v) { return *(const u4 *)((const char *)&sh_v[buf][32 * y * 8] + (v_base ^ (32 * v))); };
+    auto run_of = [](int z) { return 32 * (z / 4) + 16 * (z / 2 & 1) + 4 * (z & 1); }; // position of element 4 (z & 3) of sc[z / 4], less 8 hh
+
+    f16v acc[DT] = {}, sc[2];
+    Frag pf[4][NP]; // weights of positions 16 v + 8 hh + j
     float off = -kInf, sum = 0.f;
-    Pages here{}, next{};
-    if (begin < end) {
-        here = pages(begin);
-        load(begin, here, 0);
-        if (begin + 1 < end) next = pages(begin + 1);
-        stage(0);
-        __syncthreads();
-    }
-    for (int x = begin; x < end; x++) {
-        const int buf = (x - begin) & 1, t0 = range.tile(x) * TT;
-        const bool more = x + 1 < end;
-        const Pages now_here = here;
-        if (more) {
-            load(x + 1, next, buf ^ 1);
-            here = next;
-            if (x + 2 < end) next = pages(x + 2);
+    // The weighted sum of one tile and the scores of the other, 2 x 32 positions.  Each of these products wants 16 bytes of LDS per lane, as long on their way as four
+    // products take and no less of LDS's time than of the matrix cores': they are asked for kDeep products ahead.
+    auto products = [&](auto with_values, int xv, auto with_scores, int xs) {
+        constexpr int V = decltype(with_values)::value ? 4 * DT : 0, K = decltype(with_scores)::value ? 2 * KS : 0, kDeep = 6;
+        const int vb = (xv - begin) % 3, kb = (xs - begin) & 1;
+        auto at = [&](int z) { return z < V ? v_at(vb, z % DT, z / DT) : k_at(kb, (z - V) / 2, (z - V) % 2); };
+        if (K) sc[0] = sc[1] = f16v{};
+        u4 ring[kDeep];
+#pragma unroll
+        for (int z = 0; z < kDeep; z++) ring[z] = at(z);
+#pragma unroll
+        for (int z = 0; z < V + K; z++) {
+            const Frag f = __builtin_bit_cast(Frag, ring[z % kDeep]);
+            if (z + kDeep < V + K) ring[z % kDeep] = at(z + kDeep);
+#pragma unroll
+            for (int y = 0; y < NP; y++) {
+                if (z < V) acc[z % DT] = mfma32(f, pf[z / DT][y], acc[z % DT]);
+                else sc[(z - V) % 2] = mfma32(f, q[(z - V) / 2][y], sc[(z - V) % 2]);
+            }
         }
-        const bool none = w_last < t0 || (a.window && t0 + TT - 1 <= w_first - a.window && t0 >= a.sinks);
-        if (!none) {
-            // scores of 2 x 32 positions: position 32 y + 16 s + 8 hh + 4 (b & 1) + r in element 4 b + r, b = 2 s + (b & 1)
-            f16v sc[2] = {};
-            const int kr_row = (n & 0x13) | (n & 4) << 1 | (n & 8) >> 1;
+        __builtin_amdgcn_sched_group_barrier(0x100, kDeep, 0);
 #pragma unroll
-            for (int k = 0; k < KS; k++)
+        for (int z = 0; z < V + K; z++) {
+            __builtin_amdgcn_sched_group_barrier(0x8, NP, 0);
+            if (z + kDeep < V + K) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+    };
+    // Weights of tile x from its scores.
+    auto weights = [&](int x, int bits_there) {
+        const int vb = (x - begin) % 3, t0 = range.tile(x) * TT;
+        const bool whole = bits_there == 15 && all_visible(t0, w_first, w_last);
+        if (C::kEight) {
 #pragma unroll
-                for (int y = 0; y < 2; y++) {
-                    const Frag f = __builtin_bit_cast(Frag, sh_k[buf][piece_at<PK>(32 * y + kr_row, 2 * k + hh)]);
+            for (int z = 0; z < 8; z++) {
+                const f4 ks = *(const f4 *)&sh_ks[vb][run_of(z) + 8 * hh];
 #pragma unroll
-                    for (int z = 0; z < NP; z++) sc[y] = mfma32(f, q[k][z], sc[y]);
+                for (int r = 0; r < 4; r++) sc[z / 4][4 * (z & 3) + r] *= ks[r];
+            }
+        }
+        float top_v = 0.f; // the largest scale of the values that the row sees
+        if (whole) {
+            if (C::kEight) top_v = sh_top[vb];
+        } else {
+#pragma unroll
+            for (int z = 0; z < 8; z++) {
+                const int t = run_of(z) + 8 * hh;
+                const bool here = bits_there >> (2 * (z / 4) + (z / 2 & 1)) & 1; // t / 16
+                f4 vs = {};
+                if (C::kEight) vs = *(const f4 *)&sh_vs[vb][t];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const bool see = here & seen(t0 + t + r);
+                    sc[z / 4][4 * (z & 3) + r] = see ? sc[z / 4][4 * (z & 3) + r] : -kInf;
+                    if (C::kEight) top_v = fmaxf(top_v, see ? vs[r] : 0.f);
                 }
-            const bool whole = (now_here.p[0] | now_here.p[1] | now_here.p[2] | now_here.p[3]) >= 0 && all_visible(t0);
-            auto run_of = [](int z) { return 32 * (z / 4) + 16 * (z / 2 & 1) + 4 * (z & 1); }; // of element 4 (z & 3) of sc[z / 4], less 8 hh
+            }
             if (C::kEight) {
-#pragma unroll
-                for (int z = 0; z < 8; z++) {
-                    const f4 ks = *(const f4 *)&sh_ks[buf][run_of(z) + 8 * hh];
-#pragma unroll
-                    for (int r = 0; r < 4; r++) sc[z / 4][4 * (z & 3) + r] *= ks[r];
-                }
+                const lanes::Both v2 = lanes::both32(top_v);
+                top_v = fmaxf(v2.lo, v2.hi);
             }
-            float top_v = 0.f; // the largest scale of the values that the row sees
-            if (whole) {
-                if (C::kEight) top_v = sh_top[buf];
-            } else {
+        }
+        float mx = -kInf;
 #pragma unroll
-                for (int z = 0; z < 8; z++) {
-                    const int t = run_of(z) + 8 * hh;
-                    const bool here = now_here.p[2 * (z / 4) + (z / 2 & 1)] >= 0; // t / 16
-                    f4 vs = {};
-                    if (C::kEight) vs = *(const f4 *)&sh_vs[buf][t];
+        for (int z = 0; z < 8; z++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const bool see = here && visible(a, t0 + t + r, pos);
-                        sc[z / 4][4 * (z & 3) + r] = see ? sc[z / 4][4 * (z & 3) + r] : -kInf;
-                        if (C::kEight) top_v = fmaxf(top_v, see ? vs[r] : 0.f);
-                    }
-                }
-                if (C::kEight) {
-                    const lanes::Both v2 = lanes::both32(top_v);
-                    top_v = fmaxf(v2.lo, v2.hi);
-                }
+            for (int r = 0; r < 4; r++) mx = fmaxf(mx, sc[z / 4][4 * (z & 3) + r]);
+        const lanes::Both m2 = lanes::both32(mx);
+        float top = fmaxf(m2.lo, m2.hi) * c;
+        if (C::kEight) top += above(top_v);
+        const float f = follow(off, top);
+        if (__ballot(f != 1.f)) {
+#pragma unroll
+            for (int y = 0; y < DT; y++) acc[y] *= f;
+            sum *= f;
+        }
+        const float now = off == -kInf ? 0.f : off; // nothing seen yet: every weight is exp2(-inf)
+#pragma unroll
+        for (int v = 0; v < 4; v++) { // positions 16 v + 8 hh + j
+            f8 p;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                p[j] = __builtin_amdgcn_exp2f(fmaf(sc[v / 2][8 * (v & 1) + j], c, -now));
+                sum += p[j];
             }
-            float mx = -kInf;
+            if (C::kEight) {
+                const f4 v0 = *(const f4 *)&sh_vs[vb][16 * v + 8 * hh], v1 = *(const f4 *)&sh_vs[vb][16 * v + 8 * hh + 4];
 #pragma unroll
-            for (int z = 0; z < 8; z++)
+                for (int j = 0; j < 8; j++) p[j] *= j < 4 ? v0[j % 4] : v1[j % 4];
+                if (!whole) // the scale of a row that is not seen may be NaN
 #pragma unroll
-                for (int r = 0; r < 4; r++) mx = fmaxf(mx, sc[z / 4][4 * (z & 3) + r]);
-            const lanes::Both m2 = lanes::both32(mx);
-            float top = fmaxf(m2.lo, m2.hi) * c;
-            if (C::kEight) top += above(top_v);
-            const float f = follow(off, top);
-            if (__ballot(f != 1.f)) {
-#pragma unroll
-                for (int y = 0; y < DT; y++) acc[y] *= f;
-                sum *= f;
+                    for (int j = 0; j < 8; j++) p[j] = sc[v / 2][8 * (v & 1) + j] == -kInf ? 0.f : p[j];
             }
-            const float now = off == -kInf ? 0.f : off; // nothing seen yet: every weight is exp2(-inf)
-            bool odd = false; // a value that is not finite where some row may not see it
-#pragma unroll
-            for (int v = 0; v < 4; v++) { // positions 16 v + 8 hh + j
-                f8 p;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int z = 2 * v + j / 4;
-                    p[j] = __builtin_amdgcn_exp2f(fmaf(sc[z / 4][4 * (z & 3) + j % 4], c, -now));
-                    sum += p[j];
-                }
-                if (C::kEight) {
-                    const f4 v0 = *(const f4 *)&sh_vs[buf][16 * v + 8 * hh], v1 = *(const f4 *)&sh_vs[buf][16 * v + 8 * hh + 4];
-#pragma unroll
-                    for (int j = 0; j < 8; j++) p[j] *= j < 4 ? v0[j % 4] : v1[j % 4];
-                    if (!whole) // the scale of a row that is not seen may be NaN
-#pragma unroll
-                        for (int j = 0; j < 8; j++) p[j] = sc[v / 2][8 * (v & 1) + j] == -kInf ? 0.f : p[j];
-                }
-                Frag pf[NP];
-                pieces<Frag, typename C::One, NP>(p, pf);
-#pragma unroll
-                for (int y = 0; y < DT; y++) {
-                    u4 bits = sh_v[buf][piece_at<8>(32 * y + n, 2 * v + hh)];
-                    if (!C::kEight && !whole) bits = finite<KV>(bits, odd);
-                    const Frag fr = __builtin_bit_cast(Frag, bits);
-#pragma unroll
-                    for (int z = 0; z < NP; z++) acc[y] = mfma32(fr, pf[z], acc[y]);
-                }
-            }
-            if (!C::kEight && __ballot(odd)) { // added one by one, to the rows that see them
-                const uint16_t *cells = (const uint16_t *)&sh_v[buf][0];
+            pieces<Frag, typename C::One, NP>(p, pf[v]);
+        }
+        if (!C::kEight && sh_odd[vb] == x) {
 #pragma unroll 1
-                for (int y = 0; y < TT; y++) {
-                    const int page = y < 32 ? (y < 16 ? now_here.p[0] : now_here.p[1]) : (y < 48 ? now_here.p[2] : now_here.p[3]);
-                    if (page < 0 || !visible(a, t0 + y, pos)) continue;
-                    int half = hh; // unknown, so that 64 places are not worked out ahead of the loop
-                    asm volatile("" : "+v"(half));
+            for (int y = 0; y < TT; y++) {
+                const int t = t0 + y, page = kv::page_at(b, l.n_pages, i, t >> l.page_shift);
+                if (page < 0 || !seen(t)) continue;
+                int half = hh; // unknown, so that 64 places are not worked out ahead of the loop
+                asm volatile("" : "+v"(half));
+                const uint16_t *cells = (const uint16_t *)l.v + (((int64_t)page * l.n_heads + h) * D * size + (t & (size - 1)));
 #pragma unroll
-                    for (int z = 0; z < DT; z++) {
+                for (int z = 0; z < DT; z++) {
 #pragma unroll
-                        for (int r = 0; r < 16; r++) {
-                            const int d = 32 * z + 8 * (r / 4) + 4 * half + r % 4;
-                            const uint16_t bits = cells[8 * piece_at<8>(d, y >> 3) + (y & 7)];
-                            const float v = KV == L2_KV_F16 ? (float)__builtin_bit_cast(_Float16, bits) : kv::bf16_float(bits);
-                            if (!(fabsf(v) < kInf)) acc[z][r] += v;
-                        }
-                        asm volatile("" ::: "memory");
+                    for (int r = 0; r < 16; r++) {
+                        const uint16_t bits = cells[(int64_t)(32 * z + 8 * (r / 4) + 4 * half + r % 4) * size];
+                        const float v = KV == L2_KV_F16 ? (float)__builtin_bit_cast(_Float16, bits) : kv::bf16_float(bits);
+                        if (!(fabsf(v) < kInf)) acc[z][r] += v;
                     }
+                    asm volatile("" ::: "memory");
                 }
             }
         }
-        if (more) stage(buf ^ 1);
-        __syncthreads();
+    };
+
+    if (begin < end) {
+        constexpr std::true_type yes{};
+        constexpr std::false_type no{};
+        ask_pages(begin);
+        ask(begin, 0);
+        put(begin, 0);
+        if (late) ask(begin, 1);
+        barrier();
+        if (late) {
+            if (C::kEight) put(begin, 1);
+            barrier();
+        }
+        if (C::kEight || !late) ask(begin, late ? 2 : 1);
+        products(no, begin, yes, begin);
+        if (!C::kEight && late) put(begin, 1);
+        barrier();
+        for (int x = begin; x + 1 < end; x++) { // (left in its middle, the loop has the accumulators in registers twice)
+            // the vector ALUs' step
+            if (!C::kEight && late) ask(x, 2);
+            weights(x, ahead & 15);
+            if (C::kEight || !late) put(x, late ? 2 : 1);
+            ahead >>= 4;
+            barrier();
+            // the matrix cores'
+            if (C::kEight || !late) ask(x + 1, late ? 2 : 1);
+            products(yes, x, yes, x + 1);
+            if (!C::kEight && late) put(x + 1, 1);
+            barrier();
+        }
+        weights(end - 1, ahead & 15);
+        barrier();
+        products(yes, end - 1, no, end - 1);
+        if (!late) barrier();
     }
     const lanes::Both s2 = lanes::both32(sum);
     sum = s2.lo + s2.hi;
@@ -821,17 +875,15 @@ void kv_attention_plan(const KvLayer &l, int kv_type, const l2_kvbatch &b, const
     // A single sequence is the one kernel's or the other's; several may be some of each.
     plan->narrow_rows = group > kNarrowRows || (plan->wide && seqs == 1) ? 0 : kNarrowRows / group * group;
     plan->narrow_splits = plan->wide_splits = 1;
-    const char *e1 = getenv("KVA"), *e2 = getenv("KVB");
     if (plan->narrow_rows)
-        parts_of(seqs * l.n_heads, (e1 ? atoi(e1) : 2) * cu_count(), tiles_seen(kv_type <= L2_KV_E4M3 ? 64 : 32, kNarrowRows), (e2 ? atoi(e2) : 2) * kNarrowWaves, &plan->narrow_splits,
+        parts_of(seqs * l.n_heads, 2 * cu_count(), tiles_seen(kv_type <= L2_KV_E4M3 ? 64 : 32, kNarrowRows), kNarrowWaves, &plan->narrow_splits,
                  &plan->narrow_per);
     // row tiles of all sequences, at most: their whole ones, and a last one of each that has more rows than the narrow kernel takes
     const int64_t all = (int64_t)b.n_rows * group;
-    plan->wide_tiles = (int)std::min<int64_t>(all / kWideRows + std::min<int64_t>(seqs, all / (plan->narrow_rows + 1)), 1 << 26);
-    // blocks for every CU's room: two, or one of those with more registers
-    const int room = pieces_index(kv_type, a.type) == 0 ? 2 : 1;
+    const int64_t tile = kWideRows;
+    plan->wide_tiles = (int)std::min<int64_t>(all / tile + std::min<int64_t>(seqs, all / (plan->narrow_rows + 1)), 1 << 26);
     if (plan->wide)
-        parts_of(std::max<int64_t>(all / kWideRows, 1) * l.n_heads, room * cu_count(), tiles_seen(64, (kWideRows + group - 1) / group), 4, &plan->wide_splits,
+        parts_of(std::max<int64_t>(all / tile, 1) * l.n_heads, cu_count(), tiles_seen(64, (tile + group - 1) / group), 4, &plan->wide_splits,
                  &plan->wide_per);
     plan->stride = std::max(plan->narrow_splits, plan->wide_splits);
     plan->workspace = plan->stride > 1 ? (size_t)b.n_rows * a.n_heads * plan->stride * (l.head_size * 4 + 8) : 0;
