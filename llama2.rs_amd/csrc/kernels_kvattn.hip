@@ -382,10 +382,12 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
     }
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-    v = lanes::rows_max(v);
-    for (int o = 8; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+__device__ __forceinline__ float wave_max(float v) { // lanes 1, then 2 away; the other four, the other eight of a row; the other rows
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true)));
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true)));
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xF, 0xF, true)));
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xF, 0xF, true)));
+    return lanes::rows_max(v);
 }
 
 // Joins the parts of each query row: a block per row and head, its waves parts in turn.  NARROW: block x has row x % most of sequence x / most, most rows at the most;
@@ -445,9 +447,6 @@ __device__ __forceinline__ int piece_at(int r, int x) {
 __device__ __forceinline__ kv::Seq uniform(const kv::Seq &s) {
     return {__builtin_amdgcn_readfirstlane(s.first), __builtin_amdgcn_readfirstlane(s.rows), __builtin_amdgcn_readfirstlane(s.length)};
 }
-// A word of memory that nothing writes while the kernel runs, at an address that is the same in every lane.
-__device__ __forceinline__ int uniform_load(const int32_t *p) { return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)p; }
-
 // From memory (a base that is the same in every lane, and an offset of each, or each lane's address) into LDS, lane l's 16 bytes to `lds` + 16 l.  The compiler
 // does not know of these loads: wait_lds_loads() before the barrier behind which they are read.
 __device__ __forceinline__ void lds_load(uint32_t lds, const char *base, uint32_t off) {
@@ -468,7 +467,7 @@ __device__ __forceinline__ void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n
 // runs of 16 positions, each in one page; their addresses are computed once per wave.
 //
 // The two waves of a SIMD take turns: while the first four waves have the matrix cores (the weighted sum of the tile before, then the scores of this one), the
-// last four have the vector ALUs (exponentials, the next tile's conversion), half a tile behind, and the barriers between keep it so.  Left to themselves, waves of
+// last four have the vector ALUs (exponentials), half a tile behind, and the barriers between keep it so.  Left to themselves, waves of
 // two blocks had either unit busy for 28 and 52 % of the time, hardly ever together.  In steps of half a tile, 0 the first: the first four do the products of tile i in step 2 i
 // and its exponentials in 2 i + 1, the others each a step later.  So keys of tile i are read in steps 2 i and 2 i + 1, its values in 2 i + 2 and 2 i + 3, its scales in 2 i + 1 and 2 i + 2;
 // with two places for keys and three for the rest, tile i + 1 may be written from step 2 i on, and is there before 2 i + 2.
@@ -577,14 +576,15 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
 
     u4 kr[LOADS], vr[LOADS];
     float scale = 0.f;
-    // Entries of the table for the tile that is asked for next: of the runs of this wave's pieces of K, and of this lane's piece of V.  What lies behind the table is
+    // Entries of the table for the tile that is asked for next: of the runs of this wave's pieces of K (the same in every lane, but not by a scalar load, which the
+    // compiler would put off until they are needed), and of this lane's piece of V.  What lies behind the table is
     // behind every position too.
     int k_page[LOADS], v_page = -1;
     const int32_t *table = b.pages + (int64_t)i * b.max_pages;
     auto ask_pages = [&](int x) {
         const int t0 = range.tile(x) * TT;
 #pragma unroll
-        for (int y = 0; y < LOADS; y++) k_page[y] = uniform_load(table + min((t0 + (w * 1024 + y * 16 * kWideThreads) / RUN * 16) >> l.page_shift, b.max_pages - 1));
+        for (int y = 0; y < LOADS; y++) k_page[y] = table[min((t0 + (w * 1024 + y * 16 * kWideThreads) / RUN * 16) >> l.page_shift, b.max_pages - 1)];
         v_page = table[min((t0 + 16 * v_run) >> l.page_shift, b.max_pages - 1)];
     };
     const int64_t page_cells = (int64_t)l.n_heads * size * D * C::kSize; // bytes of a page's K (V)
@@ -604,7 +604,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
             const char *v_at = v_from + (int64_t)(is ? v_page : 0) * page_cells + ((t0 + 16 * v_run) & (size - 1)) * C::kSize;
 #pragma unroll
             for (int y = 0; y < LOADS; y++) {
-                const int page = (uint32_t)k_page[y] < (uint32_t)l.n_pages ? k_page[y] : 0, run = (w * 1024 + y * 16 * kWideThreads) / RUN;
+                const int entry = __builtin_amdgcn_readfirstlane(k_page[y]), page = (uint32_t)entry < (uint32_t)l.n_pages ? entry : 0, run = (w * 1024 + y * 16 * kWideThreads) / RUN;
                 const char *at = k_from + (int64_t)page * page_cells + ((t0 + 16 * run) & (size - 1)) * (D * C::kSize);
                 if constexpr (C::kEight) kr[y] = *(const u4 *)(at + k_off);
                 else lds_load(lds_k + (kb * TT * PK + y * kWideThreads) * 16, at, k_off);
@@ -786,13 +786,19 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
         ask_pages(begin);
         ask(begin, 0);
         put(begin, 0);
-        if (late) ask(begin, 1);
+        if (C::kEight || late) ask(begin, 1);
         barrier();
-        if (late) {
-            if (C::kEight) put(begin, 1);
-            barrier();
-        }
-        if (C::kEight || !late) ask(begin, late ? 2 : 1);
+        if (late) barrier();
+        // before the products of tile x: what is behind it
+        auto ahead_of = [&](int x) {
+            if constexpr (C::kEight) {
+                put(x, 1);
+                ask(x, 2);
+            } else if (!late) {
+                ask(x, 1);
+            }
+        };
+        ahead_of(begin);
         products(no, begin, yes, begin);
         if (!C::kEight && late) put(begin, 1);
         barrier();
@@ -800,11 +806,11 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
             // the vector ALUs' step
             if (!C::kEight && late) ask(x, 2);
             weights(x, ahead & 15);
-            if (C::kEight || !late) put(x, late ? 2 : 1);
+            if (!C::kEight && !late) put(x, 1);
             ahead >>= 4;
             barrier();
             // the matrix cores'
-            if (C::kEight || !late) ask(x + 1, late ? 2 : 1);
+            ahead_of(x + 1);
             products(yes, x, yes, x + 1);
             if (!C::kEight && late) put(x + 1, 1);
             barrier();
