@@ -382,6 +382,20 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
     }
 }
 
+// What lane M of a row of 16 lanes has, for every lane of the row.
+template <int M>
+__device__ __forceinline__ float scale_at(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x150 + M, 0xF, 0xF, true));
+}
+template <class F, int... I>
+__device__ __forceinline__ void each_of(const F &f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each(const F &f) {
+    each_of(f, std::make_integer_sequence<int, N>{});
+}
+
 __device__ __forceinline__ float wave_max(float v) { // lanes 1, then 2 away; the other four, the other eight of a row; the other rows
     v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true)));
     v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true)));
@@ -621,6 +635,18 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
         }
         if (x + 1 < end) ask_pages(x + 1);
     };
+    // Writes what has come of tile x to LDS, as 16-bit numbers.
+    auto to_lds = [&](int x) {
+        const int kb = (x - begin) & 1, vb = (x - begin) % 3;
+#pragma unroll
+        for (int y = 0; y < LOADS; y++) {
+            const int p = tid + kWideThreads * y, kr_row = p * 16 / (D * C::kSize), kr_x = p % (D * C::kSize / 16), row = v_row + kWideThreads / COL16 * y;
+            sh_k[kb][piece_at<PK>(kr_row, 2 * kr_x)] = __builtin_bit_cast(u4, C::frag(kr[y], 0));
+            sh_k[kb][piece_at<PK>(kr_row, 2 * kr_x + 1)] = __builtin_bit_cast(u4, C::frag(kr[y], 1));
+            sh_v[vb][piece_at<8>(row, 2 * v_x)] = __builtin_bit_cast(u4, C::frag(vr[y], 0));
+            sh_v[vb][piece_at<8>(row, 2 * v_x + 1)] = __builtin_bit_cast(u4, C::frag(vr[y], 1));
+        }
+    };
     // Writes the tile `by` tiles behind x, asked for before, to LDS.  16-bit cells are there already: where a row may not see all of the tile, values that are not finite
     // are taken out (and added to the rows that do see them, one by one).
     auto put = [&](int x, int by) {
@@ -639,14 +665,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
             }
             return;
         }
-#pragma unroll
-        for (int y = 0; y < LOADS; y++) {
-            const int p = tid + kWideThreads * y, kr_row = p * 16 / (D * C::kSize), kr_x = p % (D * C::kSize / 16), row = v_row + kWideThreads / COL16 * y;
-            sh_k[kb][piece_at<PK>(kr_row, 2 * kr_x)] = __builtin_bit_cast(u4, C::frag(kr[y], 0));
-            sh_k[kb][piece_at<PK>(kr_row, 2 * kr_x + 1)] = __builtin_bit_cast(u4, C::frag(kr[y], 1));
-            sh_v[vb][piece_at<8>(row, 2 * v_x)] = __builtin_bit_cast(u4, C::frag(vr[y], 0));
-            sh_v[vb][piece_at<8>(row, 2 * v_x + 1)] = __builtin_bit_cast(u4, C::frag(vr[y], 1));
-        }
+        to_lds(x);
         if (w < 2) (w ? sh_vs : sh_ks)[vb][lane] = scale;
         if (w == 1) {
             const float most = wave_max(scale);
@@ -691,35 +710,33 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
             if (z + kDeep < V + K) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
     };
+    // A tile's scales, of which a lane wants 32 and every lane of its half the same: lane m of a row of 16 has those of elements m of sc[0] and sc[1].
+    float ks[2], vs[2];
+    auto ask_scales = [&](const float *from, float *to) {
+        const float *at = from + (lane & 3) + (lane & 4) + 2 * (lane & 8) + 8 * hh; // run_of(m / 4) + m % 4
+        to[0] = at[0];
+        to[1] = at[32];
+    };
     // Weights of tile x from its scores.
     auto weights = [&](int x, int bits_there) {
         const int vb = (x - begin) % 3, t0 = range.tile(x) * TT;
         const bool whole = bits_there == 15 && all_visible(t0, w_first, w_last);
-        if (C::kEight) {
-#pragma unroll
-            for (int z = 0; z < 8; z++) {
-                const f4 ks = *(const f4 *)&sh_ks[vb][run_of(z) + 8 * hh];
-#pragma unroll
-                for (int r = 0; r < 4; r++) sc[z / 4][4 * (z & 3) + r] *= ks[r];
-            }
+        if constexpr (C::kEight) {
+            ask_scales(sh_vs[vb], vs);
+            each<32>([&](auto at) { sc[at / 16][at % 16] *= scale_at<at % 16>(ks[at / 16]); });
         }
         float top_v = 0.f; // the largest scale of the values that the row sees
         if (whole) {
             if (C::kEight) top_v = sh_top[vb];
         } else {
-#pragma unroll
-            for (int z = 0; z < 8; z++) {
+            each<32>([&](auto at) {
+                constexpr int z = at / 4, r = at % 4;
                 const int t = run_of(z) + 8 * hh;
-                const bool here = bits_there >> (2 * (z / 4) + (z / 2 & 1)) & 1; // t / 16
-                f4 vs = {};
-                if (C::kEight) vs = *(const f4 *)&sh_vs[vb][t];
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const bool see = here & seen(t0 + t + r);
-                    sc[z / 4][4 * (z & 3) + r] = see ? sc[z / 4][4 * (z & 3) + r] : -kInf;
-                    if (C::kEight) top_v = fmaxf(top_v, see ? vs[r] : 0.f);
-                }
-            }
+                const float v_scale = C::kEight ? scale_at<at % 16>(vs[at / 16]) : 0.f; // (by all lanes of the row)
+                const bool here = bits_there >> (2 * (z / 4) + (z / 2 & 1)) & 1, see = here & seen(t0 + t + r); // run t / 16
+                sc[z / 4][4 * (z & 3) + r] = see ? sc[z / 4][4 * (z & 3) + r] : -kInf;
+                if constexpr (C::kEight) top_v = fmaxf(top_v, see ? v_scale : 0.f);
+            });
             if (C::kEight) {
                 const lanes::Both v2 = lanes::both32(top_v);
                 top_v = fmaxf(v2.lo, v2.hi);
@@ -740,24 +757,26 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
             sum *= f;
         }
         const float now = off == -kInf ? 0.f : off; // nothing seen yet: every weight is exp2(-inf)
-#pragma unroll
-        for (int v = 0; v < 4; v++) { // positions 16 v + 8 hh + j
+        each<4>([&](auto v) { // positions 16 v + 8 hh + j
             f8 p;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 p[j] = __builtin_amdgcn_exp2f(fmaf(sc[v / 2][8 * (v & 1) + j], c, -now));
                 sum += p[j];
             }
-            if (C::kEight) {
-                const f4 v0 = *(const f4 *)&sh_vs[vb][16 * v + 8 * hh], v1 = *(const f4 *)&sh_vs[vb][16 * v + 8 * hh + 4];
-#pragma unroll
-                for (int j = 0; j < 8; j++) p[j] *= j < 4 ? v0[j % 4] : v1[j % 4];
-                if (!whole) // the scale of a row that is not seen may be NaN
+            if constexpr (C::kEight) {
+                each<8>([&](auto j) { p[(int)j] *= scale_at<8 * (v & 1) + j>(vs[v / 2]); });
+                if (NP > 1 && !whole) // the scale of a row that is not seen may be NaN
 #pragma unroll
                     for (int j = 0; j < 8; j++) p[j] = sc[v / 2][8 * (v & 1) + j] == -kInf ? 0.f : p[j];
             }
             pieces<Frag, typename C::One, NP>(p, pf[v]);
-        }
+        });
+        if (C::kEight && NP == 1 && !whole) // as above, but behind the loop, which then is a single run of instructions (more pieces leave no registers for it)
+#pragma unroll
+            for (int v = 0; v < 4; v++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) pf[v][0][j] = sc[v / 2][8 * (v & 1) + j] == -kInf ? (typename C::One)0.f : pf[v][0][j];
         if (!C::kEight && sh_odd[vb] == x) {
 #pragma unroll 1
             for (int y = 0; y < TT; y++) {
@@ -800,6 +819,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
         };
         ahead_of(begin);
         products(no, begin, yes, begin);
+        if (C::kEight) ask_scales(sh_ks[0], ks);
         if (!C::kEight && late) put(begin, 1);
         barrier();
         for (int x = begin; x + 1 < end; x++) { // (left in its middle, the loop has the accumulators in registers twice)
@@ -812,6 +832,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
             // the matrix cores'
             ahead_of(x + 1);
             products(yes, x, yes, x + 1);
+            if (C::kEight) ask_scales(sh_ks[(x + 1 - begin) % 3], ks);
             if (!C::kEight && late) put(x + 1, 1);
             barrier();
         }
@@ -888,8 +909,8 @@ void kv_attention_plan(const KvLayer &l, int kv_type, const l2_kvbatch &b, const
     const int64_t all = (int64_t)b.n_rows * group;
     const int64_t tile = kWideRows;
     plan->wide_tiles = (int)std::min<int64_t>(all / tile + std::min<int64_t>(seqs, all / (plan->narrow_rows + 1)), 1 << 26);
-    if (plan->wide)
-        parts_of(std::max<int64_t>(all / tile, 1) * l.n_heads, cu_count(), tiles_seen(64, (tile + group - 1) / group), 4, &plan->wide_splits,
+    if (plan->wide) // (as many tiles as there would be if each sequence's last one were half full)
+        parts_of(std::min<int64_t>((all + seqs * (tile / 2) + tile / 2 - 1) / tile, plan->wide_tiles) * l.n_heads, cu_count(), tiles_seen(64, (tile + group - 1) / group), 4, &plan->wide_splits,
                  &plan->wide_per);
     plan->stride = std::max(plan->narrow_splits, plan->wide_splits);
     plan->workspace = plan->stride > 1 ? (size_t)b.n_rows * a.n_heads * plan->stride * (l.head_size * 4 + 8) : 0;
