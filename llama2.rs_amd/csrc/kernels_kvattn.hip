@@ -686,7 +686,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
     // The weighted sum of one tile and the scores of the other, 2 x 32 positions.  Each of these products wants 16 bytes of LDS per lane, as long on their way as four
     // products take and no less of LDS's time than of the matrix cores': they are asked for kDeep products ahead.
     auto products = [&](auto with_values, int xv, auto with_scores, int xs) {
-        constexpr int V = decltype(with_values)::value ? 4 * DT : 0, K = decltype(with_scores)::value ? 2 * KS : 0, kDeep = 6;
+        constexpr int V = decltype(with_values)::value ? 4 * DT : 0, K = decltype(with_scores)::value ? 2 * KS : 0, kDeep = NP == 1 ? 6 : 5 - NP;
         const int vb = (xv - begin) % 3, kb = (xs - begin) & 1;
         auto at = [&](int z) { return z < V ? v_at(vb, z % DT, z / DT) : k_at(kb, (z - V) / 2, (z - V) % 2); };
         if (K) sc[0] = sc[1] = f16v{};
