@@ -903,7 +903,7 @@ void kv_attention_plan(const KvLayer &l, int kv_type, const l2_kvbatch &b, const
     plan->narrow_rows = group > kNarrowRows || (plan->wide && seqs == 1) ? 0 : kNarrowRows / group * group;
     plan->narrow_splits = plan->wide_splits = 1;
     if (plan->narrow_rows)
-        parts_of(seqs * l.n_heads, 2 * cu_count(), tiles_seen(kv_type <= L2_KV_E4M3 ? 64 : 32, kNarrowRows), kNarrowWaves, &plan->narrow_splits,
+        parts_of((plan->wide ? (seqs + 1) / 2 : seqs) * l.n_heads, 2 * cu_count(), tiles_seen(kv_type <= L2_KV_E4M3 ? 64 : 32, kNarrowRows), kNarrowWaves, &plan->narrow_splits,
                  &plan->narrow_per);
     // row tiles of all sequences, at most: their whole ones, and a last one of each that has more rows than the narrow kernel takes
     const int64_t all = (int64_t)b.n_rows * group;
