@@ -396,13 +396,14 @@ __device__ __forceinline__ void each(const F &f) {
     each_of(f, std::make_integer_sequence<int, N>{});
 }
 
-__device__ __forceinline__ float wave_max(float v) { // lanes 1, then 2 away; the other four, the other eight of a row; the other rows
+__device__ __forceinline__ float row_max(float v) { // of a row of 16 lanes: 1, then 2 away; the other four, the other eight
     v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true)));
     v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true)));
     v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xF, 0xF, true)));
     v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xF, 0xF, true)));
-    return lanes::rows_max(v);
+    return v;
 }
+__device__ __forceinline__ float wave_max(float v) { return lanes::rows_max(row_max(v)); }
 
 // Joins the parts of each query row: a block per row and head, its waves parts in turn.  NARROW: block x has row x % most of sequence x / most, most rows at the most;
 // else row x.
@@ -461,16 +462,16 @@ __device__ __forceinline__ int piece_at(int r, int x) {
 __device__ __forceinline__ kv::Seq uniform(const kv::Seq &s) {
     return {__builtin_amdgcn_readfirstlane(s.first), __builtin_amdgcn_readfirstlane(s.rows), __builtin_amdgcn_readfirstlane(s.length)};
 }
-// From memory (a base that is the same in every lane, and an offset of each, or each lane's address) into LDS, lane l's 16 bytes to `lds` + 16 l.  The compiler
-// does not know of these loads: wait_lds_loads() before the barrier behind which they are read.
+// From memory (a base that is the same in every lane, and an offset of each) into LDS, lane l's 16 bytes to `lds` + 16 l.  The compiler does not know of
+// these loads: wait_lds_loads() before the barrier behind which they are read.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm" // it need not keep m0
 __device__ __forceinline__ void lds_load(uint32_t lds, const char *base, uint32_t off) {
     const uint64_t p = (uint64_t)base;
     const uint64_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)p) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32;
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(at) : "memory", "m0");
 }
-__device__ __forceinline__ void lds_load(uint32_t lds, const char *at) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(at) : "memory", "m0");
-}
+#pragma clang diagnostic pop
 __device__ __forceinline__ void wait_lds_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // A barrier that waits for this wave's LDS accesses and for no loads from memory.
@@ -489,12 +490,11 @@ template <int KV, int NP, int D>
 __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, Cut cut) {
     using C = Cells<KV>;
     using Frag = typename C::Frag;
-    constexpr int TT = 64, PK = D / 8, DT = D / 32, KS = D / 16, PIECES = TT * D * C::kSize / 16, LOADS = (PIECES + kWideThreads - 1) / kWideThreads;
-    constexpr int RUN = 16 * D * C::kSize;        // bytes of 16 rows of K
-    constexpr int COL16 = TT * C::kSize / 16;     // 16-byte pieces of the tile's part of a row of V
+    constexpr int TT = 64, PK = D / 8, DT = D / 32, KS = D / 16, LOADS = D * C::kSize / 64; // (of 16 bytes per lane: 16 positions)
     __shared__ __align__(16) u4 sh_k[2][TT * PK], sh_v[3][D * 8];
     __shared__ __align__(16) float sh_ks[3][TT], sh_vs[3][TT];
-    __shared__ float sh_top[3];
+    __shared__ __align__(16) float sh_top[3][4];
+    __shared__ uint32_t sh_there[3];
     __shared__ int sh_seq, sh_tile, sh_odd[3];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, hh = lane >> 5;
     const int group = a.n_heads / l.n_heads;
@@ -572,112 +572,94 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
     const int begin = min(split * cut.per, range.n), end = min(begin + cut.per, range.n);
     const int size = 1 << l.page_shift;
 
-    // Offsets of this thread's pieces: of K from its run's first byte, of V from the run's first position.  16-bit cells: of the piece whose place in LDS
-    // is the thread's.
-    constexpr int KX = 1024 / (16 * PK);                    // rows of K in a wave's 1024 bytes of LDS
-    const int k_row = w * KX + lane / PK, v_row = C::kEight ? tid / COL16 : tid / 8;
-    const int v_x = C::kEight ? tid % COL16 : (tid & 7) ^ (v_row >> 1 & 7);
-    const uint32_t k_off = C::kEight ? tid * 16 % RUN : ((k_row & 15) * D + 8 * (lane % PK ^ (PK == 16 ? k_row & 15 : k_row >> 1 & 7))) * 2;
-    const int v_run = C::kEight ? v_x : v_x >> 1;
-    const uint32_t v_off = (uint32_t)(v_row * size + (C::kEight ? 0 : 8 * (v_x & 1))) * C::kSize, v_step = (uint32_t)(kWideThreads / COL16) * size * C::kSize;
-    const uint32_t lds_k = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u4 *)&sh_k[0][0] + w * 1024;
-    const uint32_t lds_v = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u4 *)&sh_v[0][0] + w * 1024;
-    const bool late = w >= kWideWaves / 2; // of the last four waves
-    const bool loads = PIECES >= kWideThreads || w < PIECES / 64;
+    // The first four waves have the keys to bring, the others the values: each 16 positions of a tile, a run, which lie in one page.  A run of values is D rows of two
+    // pieces; their order in a pair changes so that the rows that an LDS read takes together meet different places.
+    const bool late = w >= kWideWaves / 2;
+    const int run = w & 3;
+    auto v_swap = [](int row) { return (row >> 2 ^ row >> 3) & 1; };
+    const uint32_t k_off = lane / PK * (D * 2) + 16 * (lane % PK ^ (PK == 16 ? lane / PK : lane / PK >> 1)); // piece `lane` of a run in LDS
+    const uint32_t v_off = lane / 2 * size * 2 + 16 * ((lane & 1) ^ v_swap(lane / 2));
+    const uint32_t lds_k = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) u4 *)&sh_k[0][0]) + run * (16 * PK * 16);
+    const uint32_t lds_v = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) u4 *)&sh_v[0][0]) + run * (2 * D * 16);
 
     // Whether every row of those from position `first` to `last` sees all of a tile whose pages are there.
     auto all_visible = [&](int t0, int first, int last) { return t0 + TT - 1 <= first && (!a.window || t0 > last - a.window || t0 + TT <= a.sinks); };
 
-    u4 kr[LOADS], vr[LOADS];
+    // The tile at hand, tile x, has place `cur` of three; where tile x + by is.
+    int cur = 0;
+    auto place = [&](int by) { return cur + by % 3 >= 3 ? cur + by % 3 - 3 : cur + by % 3; };
+    u4 raw[C::kEight ? LOADS : 1];
     float scale = 0.f;
-    // Entries of the table for the tile that is asked for next: of the runs of this wave's pieces of K (the same in every lane, but not by a scalar load, which the
-    // compiler would put off until they are needed), and of this lane's piece of V.  What lies behind the table is
-    // behind every position too.
-    int k_page[LOADS], v_page = -1;
+    bool there = false; // whether the run that was asked for has a page
+    // The entry of the table for the run that is asked for next (not by a scalar load, which the compiler would put off until the entry is needed).  What lies
+    // behind the table is behind every position too.
+    int entry = -1;
     const int32_t *table = b.pages + (int64_t)i * b.max_pages;
-    auto ask_pages = [&](int x) {
-        const int t0 = range.tile(x) * TT;
-#pragma unroll
-        for (int y = 0; y < LOADS; y++) k_page[y] = table[min((t0 + (w * 1024 + y * 16 * kWideThreads) / RUN * 16) >> l.page_shift, b.max_pages - 1)];
-        v_page = table[min((t0 + 16 * v_run) >> l.page_shift, b.max_pages - 1)];
-    };
+    auto ask_page = [&](int x) { entry = table[min((range.tile(x) * TT + 16 * run) >> l.page_shift, b.max_pages - 1)]; };
     const int64_t page_cells = (int64_t)l.n_heads * size * D * C::kSize; // bytes of a page's K (V)
-    const char *k_from = (const char *)l.k + (int64_t)h * size * D * C::kSize, *v_from = (const char *)l.v + (int64_t)h * size * D * C::kSize + v_off;
-    int ahead = 0; // which runs have a page: four bits for this tile, then for those behind it that have been asked for
-    // Asks for the tile `by` tiles behind tile x, whose pages have been asked for, and for the pages of the one behind that.
+    const char *from = (const char *)(late ? l.v : l.k) + (int64_t)h * size * D * C::kSize;
+    // Asks for this wave's run of tile x + by, whose page has been asked for, and for the page of the tile behind that.
     auto ask = [&](int x, int by) {
         x += by;
         if (x >= end) return;
-        const bool is = (uint32_t)v_page < (uint32_t)l.n_pages;
-        int runs = 15;
-        if (__ballot(!is))
-            for (int y = 0; y < 4; y++) runs &= __ballot(!is && v_run == y) ? ~(1 << y) : 15;
-        ahead |= runs << 4 * by;
-        const int t0 = range.tile(x) * TT, kb = (x - begin) & 1, vb = (x - begin) % 3;
-        if (loads) {
-            const char *v_at = v_from + (int64_t)(is ? v_page : 0) * page_cells + ((t0 + 16 * v_run) & (size - 1)) * C::kSize;
+        const int found = __builtin_amdgcn_readfirstlane(entry);
+        there = (uint32_t)found < (uint32_t)l.n_pages;
+        const int page = there ? found : 0, slot = (range.tile(x) * TT + 16 * run) & (size - 1);
+        const char *at = from + page * page_cells + slot * (late ? C::kSize : D * C::kSize);
+        if constexpr (C::kEight) {
+            const uint32_t off = late ? lane * size : lane * 16, step = late ? 64 * size : 1024;
 #pragma unroll
-            for (int y = 0; y < LOADS; y++) {
-                const int entry = __builtin_amdgcn_readfirstlane(k_page[y]), page = (uint32_t)entry < (uint32_t)l.n_pages ? entry : 0, run = (w * 1024 + y * 16 * kWideThreads) / RUN;
-                const char *at = k_from + (int64_t)page * page_cells + ((t0 + 16 * run) & (size - 1)) * (D * C::kSize);
-                if constexpr (C::kEight) kr[y] = *(const u4 *)(at + k_off);
-                else lds_load(lds_k + (kb * TT * PK + y * kWideThreads) * 16, at, k_off);
-            }
+            for (int y = 0; y < LOADS; y++) raw[y] = *(const u4 *)(at + y * step + off);
+            scale = (late ? l.v_scale : l.k_scale)[((int64_t)page * l.n_heads + h) * size + slot + (lane & 15)];
+        } else if (late) {
 #pragma unroll
-            for (int y = 0; y < LOADS; y++) {
-                if constexpr (C::kEight) vr[y] = *(const u4 *)(v_at + y * v_step);
-                else lds_load(lds_v + (vb * D * 8 + y * kWideThreads) * 16, v_at + y * v_step);
-            }
-            if (C::kEight && w < 2) { // lane y has run y of V
-                const int page = __shfl(is ? v_page : 0, lane >> 4);
-                scale = (w ? l.v_scale : l.k_scale)[((int64_t)page * l.n_heads + h) * size + ((t0 + lane) & (size - 1))];
-            }
+            for (int y = 0; y < LOADS; y++) lds_load(lds_v + place(by) * (D * 8 * 16) + y * 1024, at + y * (64 * size), v_off);
+        } else {
+            const uint32_t to = lds_k + ((x - begin) & 1) * (TT * PK * 16);
+#pragma unroll
+            for (int y = 0; y < LOADS; y++) lds_load(to + y * 1024, at + y * 1024, k_off ^ 64 * y);
         }
-        if (x + 1 < end) ask_pages(x + 1);
+        if (x + 1 < end) ask_page(x + 1);
     };
-    // Writes what has come of tile x to LDS, as 16-bit numbers.
-    auto to_lds = [&](int x) {
-        const int kb = (x - begin) & 1, vb = (x - begin) % 3;
-#pragma unroll
-        for (int y = 0; y < LOADS; y++) {
-            const int p = tid + kWideThreads * y, kr_row = p * 16 / (D * C::kSize), kr_x = p % (D * C::kSize / 16), row = v_row + kWideThreads / COL16 * y;
-            sh_k[kb][piece_at<PK>(kr_row, 2 * kr_x)] = __builtin_bit_cast(u4, C::frag(kr[y], 0));
-            sh_k[kb][piece_at<PK>(kr_row, 2 * kr_x + 1)] = __builtin_bit_cast(u4, C::frag(kr[y], 1));
-            sh_v[vb][piece_at<8>(row, 2 * v_x)] = __builtin_bit_cast(u4, C::frag(vr[y], 0));
-            sh_v[vb][piece_at<8>(row, 2 * v_x + 1)] = __builtin_bit_cast(u4, C::frag(vr[y], 1));
-        }
-    };
-    // Writes the tile `by` tiles behind x, asked for before, to LDS.  16-bit cells are there already: where a row may not see all of the tile, values that are not finite
-    // are taken out (and added to the rows that do see them, one by one).
+    // Has this wave's run of tile x + by, asked for before, in LDS.  16-bit cells get there by themselves: where a row may not see all of the tile, values that
+    // are not finite are taken out (and added to the rows that do see them, one by one).
     auto put = [&](int x, int by) {
         x += by;
-        if (x >= end || !loads) return;
-        const int kb = (x - begin) & 1, vb = (x - begin) % 3;
-        if constexpr (!C::kEight) {
+        if (x >= end) return;
+        const int kb = (x - begin) & 1, vb = place(by);
+        if (!late && lane == 0) ((uint8_t *)&sh_there[vb])[run] = there;
+        if constexpr (C::kEight) {
+#pragma unroll
+            for (int y = 0; y < LOADS; y++) {
+                const int p = 64 * y + lane, row = 16 * run + p / (PK / 2), x2 = 2 * (p % (PK / 2));
+                const Frag f0 = C::frag(raw[y], 0), f1 = C::frag(raw[y], 1);
+                u4 *to = late ? &sh_v[vb][2 * D * run + 2 * p] : &sh_k[kb][0];
+                to[late ? v_swap(p) : piece_at<PK>(row, x2)] = __builtin_bit_cast(u4, f0);
+                to[late ? v_swap(p) ^ 1 : piece_at<PK>(row, x2 + 1)] = __builtin_bit_cast(u4, f1);
+            }
+            if (lane < 16) (late ? sh_vs : sh_ks)[vb][16 * run + lane] = scale;
+            if (late) {
+                const float most = row_max(scale);
+                if (lane == 0) sh_top[vb][run] = most;
+            }
+        } else {
             wait_lds_loads();
-            if ((ahead >> 4 * by & 15) == 15 && all_visible(range.tile(x) * TT, b_first, b_last)) return;
+            if (!late || (there && all_visible(range.tile(x) * TT, b_first, b_last))) return;
 #pragma unroll
             for (int y = 0; y < LOADS; y++) {
                 bool odd = false;
-                u4 *at = &sh_v[vb][tid + kWideThreads * y];
+                u4 *at = &sh_v[vb][2 * D * run + 64 * y + lane];
                 const u4 v = finite<KV>(*at, odd);
                 if (odd) *at = v, sh_odd[vb] = x;
             }
-            return;
-        }
-        to_lds(x);
-        if (w < 2) (w ? sh_vs : sh_ks)[vb][lane] = scale;
-        if (w == 1) {
-            const float most = wave_max(scale);
-            if (lane == 0) sh_top[vb] = most;
         }
     };
 
     const int kr_row = (n & 0x13) | (n & 4) << 1 | (n & 8) >> 1;
     // (2 k + hh) ^ x is (hh ^ x) ^ 2 k: a piece's address is the first one's but for the bits of k
-    const uint32_t k_base = 16 * piece_at<PK>(kr_row, hh), v_base = 16 * piece_at<8>(n, hh);
+    const uint32_t k_base = 16 * piece_at<PK>(kr_row, hh), v_base = 16 * (2 * n + (hh ^ v_swap(n)));
     auto k_at = [&](int buf, int k, int y) { return *(const u4 *)((const char *)&sh_k[buf][32 * y * PK] + (k_base ^ (32 * k))); };
-    auto v_at = [&](int buf, int y, int v) { return *(const u4 *)((const char *)&sh_v[buf][32 * y * 8] + (v_base ^ (32 * v))); };
+    auto v_at = [&](int buf, int y, int v) { return *(const u4 *)((const char *)&sh_v[buf][2 * (D * v + 32 * y)] + v_base); };
     auto run_of = [](int z) { return 32 * (z / 4) + 16 * (z / 2 & 1) + 4 * (z & 1); }; // position of element 4 (z & 3) of sc[z / 4], less 8 hh
 
     f16v acc[DT] = {}, sc[2];
@@ -685,9 +667,8 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
     float off = -kInf, sum = 0.f;
     // The weighted sum of one tile and the scores of the other, 2 x 32 positions.  Each of these products wants 16 bytes of LDS per lane, as long on their way as four
     // products take and no less of LDS's time than of the matrix cores': they are asked for kDeep products ahead.
-    auto products = [&](auto with_values, int xv, auto with_scores, int xs) {
+    auto products = [&](auto with_values, auto with_scores, int vb, int kb) {
         constexpr int V = decltype(with_values)::value ? 4 * DT : 0, K = decltype(with_scores)::value ? 2 * KS : 0, kDeep = NP == 1 ? 6 : 5 - NP;
-        const int vb = (xv - begin) % 3, kb = (xs - begin) & 1;
         auto at = [&](int z) { return z < V ? v_at(vb, z % DT, z / DT) : k_at(kb, (z - V) / 2, (z - V) % 2); };
         if (K) sc[0] = sc[1] = f16v{};
         u4 ring[kDeep];
@@ -717,23 +698,31 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
         to[0] = at[0];
         to[1] = at[32];
     };
+    // What weights() needs of tile x + by, ahead of it.
+    uint32_t runs = 0; // which runs have a page, a byte each
+    auto look = [&](int by) {
+        runs = sh_there[place(by)];
+        if (C::kEight) ask_scales(sh_ks[place(by)], ks);
+    };
     // Weights of tile x from its scores.
-    auto weights = [&](int x, int bits_there) {
-        const int vb = (x - begin) % 3, t0 = range.tile(x) * TT;
-        const bool whole = bits_there == 15 && all_visible(t0, w_first, w_last);
+    auto weights = [&](int x) {
+        const int vb = cur, t0 = range.tile(x) * TT;
+        const uint32_t bits_there = __builtin_amdgcn_readfirstlane(runs);
+        const bool whole = bits_there == 0x01010101 && all_visible(t0, w_first, w_last);
+        const bool odd = !C::kEight && sh_odd[vb] == x;
         if constexpr (C::kEight) {
             ask_scales(sh_vs[vb], vs);
             each<32>([&](auto at) { sc[at / 16][at % 16] *= scale_at<at % 16>(ks[at / 16]); });
         }
         float top_v = 0.f; // the largest scale of the values that the row sees
         if (whole) {
-            if (C::kEight) top_v = sh_top[vb];
+            if (C::kEight) top_v = fmaxf(fmaxf(sh_top[vb][0], sh_top[vb][1]), fmaxf(sh_top[vb][2], sh_top[vb][3]));
         } else {
             each<32>([&](auto at) {
                 constexpr int z = at / 4, r = at % 4;
                 const int t = run_of(z) + 8 * hh;
                 const float v_scale = C::kEight ? scale_at<at % 16>(vs[at / 16]) : 0.f; // (by all lanes of the row)
-                const bool here = bits_there >> (2 * (z / 4) + (z / 2 & 1)) & 1, see = here & seen(t0 + t + r); // run t / 16
+                const bool here = bits_there >> 8 * (2 * (z / 4) + (z / 2 & 1)) & 1, see = here & seen(t0 + t + r); // run t / 16
                 sc[z / 4][4 * (z & 3) + r] = see ? sc[z / 4][4 * (z & 3) + r] : -kInf;
                 if constexpr (C::kEight) top_v = fmaxf(top_v, see ? v_scale : 0.f);
             });
@@ -777,7 +766,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
             for (int v = 0; v < 4; v++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) pf[v][0][j] = sc[v / 2][8 * (v & 1) + j] == -kInf ? (typename C::One)0.f : pf[v][0][j];
-        if (!C::kEight && sh_odd[vb] == x) {
+        if (odd) {
 #pragma unroll 1
             for (int y = 0; y < TT; y++) {
                 const int t = t0 + y, page = kv::page_at(b, l.n_pages, i, t >> l.page_shift);
@@ -802,43 +791,43 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
     if (begin < end) {
         constexpr std::true_type yes{};
         constexpr std::false_type no{};
-        ask_pages(begin);
+        ask_page(begin);
         ask(begin, 0);
         put(begin, 0);
         if (C::kEight || late) ask(begin, 1);
         barrier();
         if (late) barrier();
-        // before the products of tile x: what is behind it
-        auto ahead_of = [&](int x) {
+        // before the products of tile x + by: what is behind it
+        auto behind = [&](int x, int by) {
             if constexpr (C::kEight) {
-                put(x, 1);
-                ask(x, 2);
+                put(x, by + 1);
+                ask(x, by + 2);
             } else if (!late) {
-                ask(x, 1);
+                ask(x, by + 1);
             }
         };
-        ahead_of(begin);
-        products(no, begin, yes, begin);
-        if (C::kEight) ask_scales(sh_ks[0], ks);
+        behind(begin, 0);
+        products(no, yes, 0, 0);
+        look(0);
         if (!C::kEight && late) put(begin, 1);
         barrier();
         for (int x = begin; x + 1 < end; x++) { // (left in its middle, the loop has the accumulators in registers twice)
             // the vector ALUs' step
             if (!C::kEight && late) ask(x, 2);
-            weights(x, ahead & 15);
+            weights(x);
             if (!C::kEight && !late) put(x, 1);
-            ahead >>= 4;
             barrier();
             // the matrix cores'
-            ahead_of(x + 1);
-            products(yes, x, yes, x + 1);
-            if (C::kEight) ask_scales(sh_ks[(x + 1 - begin) % 3], ks);
-            if (!C::kEight && late) put(x + 1, 1);
+            behind(x, 1);
+            products(yes, yes, cur, (x + 1 - begin) & 1);
+            look(1);
+            if (!C::kEight && late) put(x, 2);
             barrier();
+            cur = place(1);
         }
-        weights(end - 1, ahead & 15);
+        weights(end - 1);
         barrier();
-        products(yes, end - 1, no, end - 1);
+        products(yes, no, cur, 0);
         if (!late) barrier();
     }
     const lanes::Both s2 = lanes::both32(sum);
