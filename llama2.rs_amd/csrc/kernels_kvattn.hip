@@ -766,6 +766,11 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
             for (int v = 0; v < 4; v++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) pf[v][0][j] = sc[v / 2][8 * (v & 1) + j] == -kInf ? (typename C::One)0.f : pf[v][0][j];
+        // here, not where the compiler would have them: between the products, which then wait for the first ones
+#pragma unroll
+        for (int v = 0; v < 4; v++)
+#pragma unroll
+            for (int y = 0; y < NP; y++) asm volatile("" : "+v"(pf[v][y]));
         if (odd) {
 #pragma unroll 1
             for (int y = 0; y < TT; y++) {
