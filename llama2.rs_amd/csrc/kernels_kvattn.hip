@@ -149,7 +149,10 @@ struct Parts {
 
 // Sequences of up to 16 query rows per kv head (new tokens x query heads of the group).  A block has one sequence, kv head and part of the positions, its
 // four waves tiles of 64 positions (32 of 16-bit cells) in turn, straight from memory into registers: 8 KB of keys and 8 KB of values, the next tile's keys
-// asked for once this one's scores are there and its values once this one's are summed.
+// asked for once this one's scores are there and its values once this one's are summed.  LDS only joins the waves: a row of V^T or K is read by one wave alone.
+// Bound by memory where the launch fills the chip: 32 sequences' next tokens, 64 heads on 8, up to 4096 positions in e4m3, 41 us (39 at a large copy's rate);
+// one behind 60001 positions of 32 heads in i8, 102 us (4.9 TB/s; at a copy's rate 108).  One behind 500 takes 11 us: two launches, and in each two or three trips
+// to memory that wait for one another.
 template <int KV, int NP, int D>
 __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, Cut cut) {
     using C = Cells<KV>;
@@ -479,13 +482,19 @@ __device__ __forceinline__ void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n
 
 // Longer chunks.  A block has 256 query rows of one sequence and kv head, a wave 32 of them; keys and values come in tiles of 64 positions through LDS, in 16
 // bits, the next one or two on their way meanwhile: codes of 8 bits into registers, to be converted once for all waves, 16-bit cells straight into LDS.  A tile is four
-// runs of 16 positions, each in one page; their addresses are computed once per wave.
+// runs of 16 positions, each in one page: four waves bring a run of keys each, the other four one of values, so that a wave has one entry of the table to ask for.
 //
 // The two waves of a SIMD take turns: while the first four waves have the matrix cores (the weighted sum of the tile before, then the scores of this one), the
 // last four have the vector ALUs (exponentials), half a tile behind, and the barriers between keep it so.  Left to themselves, waves of
 // two blocks had either unit busy for 28 and 52 % of the time, hardly ever together.  In steps of half a tile, 0 the first: the first four do the products of tile i in step 2 i
 // and its exponentials in 2 i + 1, the others each a step later.  So keys of tile i are read in steps 2 i and 2 i + 1, its values in 2 i + 2 and 2 i + 3, its scales in 2 i + 1 and 2 i + 2;
 // with two places for keys and three for the rest, tile i + 1 may be written from step 2 i on, and is there before 2 i + 2.
+//
+// Of heads of 128, a wave's products of a tile are 1024 clocks of its matrix core, per number that q and p are made of.  A step is about 2000 of 16-bit cells, where
+// the exponentials and the loads' issue are as long as the products and theirs, and 2600 of 8-bit ones, where the vector ALUs are busy throughout: each score and
+// weight is multiplied by a scale, and conversion is theirs too.  512 rows of 64 heads on 8 behind 7488 positions in i8: 180 us, 720 TFLOP/s (a large library product in
+// fp16: 1170); two prompts of 4096 and 2542, 32 heads, window 1024, bf16: 168 us, 560 TFLOP/s.  What did not pay: one conversion spread between the products
+// (+9 %), the values' wait half a tile later, scales as float4 from LDS (16 reads a tile; they now are two registers, broadcast in rows of lanes).
 template <int KV, int NP, int D>
 __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, Cut cut) {
     using C = Cells<KV>;
