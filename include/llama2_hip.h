@@ -248,7 +248,7 @@ size_t l2_kvpool_bytes(const l2_kvpool *p);
  * everything they may contain at that time (a captured call is replayed with other contents): sequence i has the rows
  * [starts[i], starts[i+1]) of the call's arrays, which are its last positions, up to lengths[i] - 1; position t of it lies in slot
  * t % page_size of page pages[i * max_pages + t / page_size].  A sequence may have no rows, or no positions; rows before starts[0]
- * and behind starts[n_seqs] are left as they are.  Entries of pages that no row has to do with are not read, and one outside
+ * and behind starts[n_seqs] are left as they are.  Entries for positions that no row sees do not matter, and one outside
  * 0..n_pages-1 is no page: what it would hold is not there.  Contents beyond the limits are cut off at them: the values of such a sequence are then
  * unspecified, but nothing outside the arrays and the pool is touched. */
 typedef struct l2_kvbatch {
@@ -273,7 +273,7 @@ int l2_kvpool_read(l2_kvpool *p, int layer, const l2_kvbatch *batch, void *k_dev
                    int64_t v_stride, void *hip_stream);
 
 /* Attention of the rows over one layer: q_dev and out_dev of `type`, [n_rows][n_heads][head_size], n_heads a multiple of the pool's (query
- * head h reads kv head h / (n_heads / n_kv_heads)); out may be q.  The row of position pos sees the positions t <= pos that have a page, with a window > 0
+ * head h reads kv head h / (n_heads / n_kv_heads)); out may be q, with its stride.  The row of position pos sees the positions t <= pos that have a page, with a window > 0
  * only those of the last `window` (t > pos - window) and of the first `sinks`.  out = sum over t of softmax(scale * q.k_t) v_t;
  * zeros where nothing is seen.  Keys and values come from the pool, those of the rows included (l2_kvpool_write first).  Scores, statistics and sums
  * are fp32; q and the softmax's weights enter the matrix cores as one 16-bit number each for 16-bit rows and as several, to within 2^-22,
@@ -302,7 +302,7 @@ int l2_kvpool_attention(l2_kvpool *p, int layer, const l2_kvbatch *batch, const 
  *   top_p:  of these, the fewest from the front whose weights reach top_p of the sum of these    (off: >= 1)
  *   min_p:  of these, those with w >= min_p (of the largest weight, which is 1)               (off: <= 0)
  * The first is always kept.  The answer is the first id, in the vocabulary's order, at which the running sum of the kept weights passes u times
- * their sum (Random::sample, src/util.rs:102-113).  A temperature of 0 (or below, or NaN) takes the first token.  Weights are whole multiples of 2^-44 and sums of them
+ * their sum (Random::sample, src/util.rs:102-113); of a u of 1 or more the last kept, and a u below 0 or NaN is 0.  A temperature of 0 (or below, or NaN) takes the first token.  Weights are whole multiples of 2^-44 and sums of them
  * exact, so a row's answer is the same in every batch and call.  NaN logits count as -infinity; a row with nothing else gets -1.  An infinite
  * logit shares everything with its equals.  vocab up to 2^19.  ids_dev is host-visible or device memory.
  * Enqueued on hip_stream without waiting; allocates nothing; may be captured (after a first call, or l2_kvpool_create, on the device).

@@ -1,6 +1,7 @@
 // Host side of the operators on a cache in pages and of sampling on device memory: handles, checks of arguments, launches.
 #include <math.h>
 
+#include <initializer_list>
 #include <new>
 
 #include "kvpool.h"
@@ -42,6 +43,11 @@ static int type_size(int type) { return type == L2_F32 ? 4 : 2; }
 
 static int check_aligned(const void *p, int type, const char *what) {
     if (reinterpret_cast<uintptr_t>(p) % type_size(type)) return l2_fail(L2_ERR_ARG, "%s is not aligned to %d bytes", what, type_size(type));
+    return L2_OK;
+}
+static int check_words(std::initializer_list<const void *> arrays) { // of 32-bit numbers, or absent
+    for (const void *p : arrays)
+        if (reinterpret_cast<uintptr_t>(p) % 4) return l2_fail(L2_ERR_ARG, "an array of 32-bit numbers at %p", p);
     return L2_OK;
 }
 
@@ -112,7 +118,7 @@ static int check_batch(const l2_kvpool *p, const l2_kvbatch *b) {
     if ((int64_t)b->max_length > (int64_t)b->max_pages * p->page_size)
         return l2_fail(L2_ERR_ARG, "%d positions do not fit %d pages of %d", b->max_length, b->max_pages, p->page_size);
     if (b->n_seqs && (!b->starts || !b->lengths || (b->max_pages && !b->pages))) return l2_fail(L2_ERR_ARG, "null argument");
-    return L2_OK;
+    return check_words({b->starts, b->lengths, b->pages});
 }
 
 static int check_layer(const l2_kvpool *p, int layer) {
@@ -185,6 +191,8 @@ extern "C" int l2_kvpool_attention(l2_kvpool *p, int layer, const l2_kvbatch *ba
     if (!q_dev || !out_dev) return l2_fail(L2_ERR_ARG, "null argument");
     L2_TRY(check_aligned(q_dev, a->type, "q"));
     L2_TRY(check_aligned(out_dev, a->type, "out"));
+    if (q_dev == out_dev && at.q_stride != at.out_stride)
+        return l2_fail(L2_ERR_ARG, "out is q, %lld and %lld from row to row", (long long)at.out_stride, (long long)at.q_stride);
     if (plan.workspace && (!workspace_dev || workspace_bytes < plan.workspace || reinterpret_cast<uintptr_t>(workspace_dev) % 16))
         return l2_fail(L2_ERR_ARG, "workspace of %zu bytes at %p (%zu wanted, aligned to 16)", workspace_bytes, workspace_dev, plan.workspace);
     L2_TRY(check_device(p->device, hip_stream));
@@ -201,6 +209,7 @@ extern "C" int l2_sample_device(const void *logits_dev, int type, int rows, int 
     if (rows == 0) return L2_OK;
     if (!logits_dev || !ids_dev || !s->u) return l2_fail(L2_ERR_ARG, "null argument");
     L2_TRY(check_aligned(logits_dev, type, "logits"));
+    L2_TRY(check_words({s->temperature, s->top_k, s->top_p, s->min_p, s->u, ids_dev}));
     L2_TRY(check_device(-1, hip_stream));
     SampleSettings how{};
     how.temperature = s->temperature, how.top_k = s->top_k, how.top_p = s->top_p, how.min_p = s->min_p, how.u = s->u;

@@ -911,7 +911,7 @@ void kv_attention_plan(const KvLayer &l, int kv_type, const l2_kvbatch &b, const
     // row tiles of all sequences, at most: their whole ones, and a last one of each that has more rows than the narrow kernel takes
     const int64_t all = (int64_t)b.n_rows * group;
     const int64_t tile = kWideRows;
-    plan->wide_tiles = (int)std::min<int64_t>(all / tile + std::min<int64_t>(seqs, all / (plan->narrow_rows + 1)), 1 << 26);
+    plan->wide_tiles = all / tile + std::min<int64_t>(seqs, all / (plan->narrow_rows + 1));
     if (plan->wide) // (as many tiles as there would be if each sequence's last one were half full)
         parts_of(std::min<int64_t>((all + seqs * (tile / 2) + tile / 2 - 1) / tile, plan->wide_tiles) * l.n_heads, cu_count(), tiles_seen(64, (tile + group - 1) / group), 4, &plan->wide_splits,
                  &plan->wide_per);
@@ -925,7 +925,7 @@ int kv_attention_launch(const KvLayer &l, int kv_type, const l2_kvbatch &b, cons
     Parts parts{(float *)workspace, nullptr};
     parts.stat = (float2 *)(parts.acc + (size_t)b.n_rows * a.n_heads * plan.stride * l.head_size);
     if (plan.wide && plan.wide_tiles) {
-        const int64_t blocks = (int64_t)plan.wide_tiles * l.n_heads * plan.wide_splits;
+        const int64_t blocks = plan.wide_tiles * l.n_heads * plan.wide_splits;
         if (blocks >= (int64_t)1 << 31) return l2_fail(L2_ERR_RANGE, "%d rows of %d heads", b.n_rows, a.n_heads);
         l2_launch(kWide[kv_type][np][big], dim3((unsigned)blocks), dim3(kWideThreads), 0, st, l, b, a, parts,
                   Cut{plan.wide_splits, plan.wide_per, plan.stride, plan.narrow_rows});

@@ -42,7 +42,7 @@ struct KvAttnPlan {
     int narrow_splits, wide_splits; // parts that positions are cut into,
     int narrow_per, wide_per;       // each of so many tiles
     int stride;                     // the larger of both: parts of a row in the workspace
-    int wide_tiles;                 // tiles of rows of the wide kernel, at most
+    int64_t wide_tiles;             // tiles of rows of the wide kernel, at most
 };
 void kv_attention_plan(const KvLayer &l, int kv_type, const l2_kvbatch &b, const KvAttention &a, KvAttnPlan *plan);
 int kv_attention_launch(const KvLayer &l, int kv_type, const l2_kvbatch &b, const KvAttention &a, const KvAttnPlan &plan, void *workspace,
