@@ -215,6 +215,36 @@ def test_long_contexts(dev, kv, t):
     c.close()
 
 
+@pytest.mark.parametrize("kv,t", [("i8", F16), ("e4m3", F32), ("f16", BF16), ("bf16", F32)])
+def test_groups_that_do_not_divide_a_tile(dev, kv, t):
+    """Chunks of several tiles of rows whose borders lie inside a token's heads, behind many tiles that all of them see."""
+    lengths, rows = [700, 1000], [111, 38]
+    c, rng = _filled(dev, kv, 32, 1, 128, lengths, seed=8, t=t)
+    q = rng.standard_normal((sum(rows), 7, 128)).astype(np.float32)
+    for window, sinks in ((0, 0), (333, 5)):
+        got = c.attend(q, rows, t, 7, window, sinks)
+        c.check(got, q, rows, t, 7, window, sinks)
+    c.close()
+
+
+@pytest.mark.parametrize("kv", ["i8", "bf16"])
+def test_pages_past_32_bits(dev, kv):
+    """Keys of more than 2^32 bytes, and sequences in their last pages."""
+    lengths, rows, heads = [600, 290], [1, 20], 32
+    c = Cache(dev, kv, 256, heads, 128, lengths, extra_pages=4200)
+    assert c.pool.nbytes > 2 * 2 ** 32
+    c.table[0] = c.n_pages - 1 - np.arange(c.max_pages)
+    c.table[1, :2] = [0, c.n_pages - 1 - c.max_pages]
+    rng = np.random.default_rng(9)
+    k, v = (rng.standard_normal((sum(lengths), heads, 128)).astype(np.float32) for _ in "kv")
+    c.fill(k, v)
+    for got, want in zip(_read(c, dev, lengths, F32), (c.k, c.v)):
+        np.testing.assert_array_equal(got, want.astype(np.float32))
+    q = rng.standard_normal((sum(rows), heads, 128)).astype(np.float32)
+    c.check(c.attend(q, rows, F32, heads), q, rows, F32, heads)
+    c.close()
+
+
 @pytest.mark.parametrize("kv,t", [("i8", F32), ("e4m3", F16), ("f16", F32), ("bf16", F32), ("bf16", F16), ("f16", BF16)])
 def test_rows_that_see_nothing(dev, kv, t):
     """No positions, no rows, more rows than positions, and rows of no sequence."""
