@@ -150,7 +150,7 @@ struct Parts {
 // Sequences of up to 16 query rows per kv head (new tokens x query heads of the group).  A block has one sequence, kv head and part of the positions, its
 // four waves tiles of 64 positions (32 of 16-bit cells) in turn, straight from memory into registers: 8 KB of keys and 8 KB of values, the next tile's keys
 // asked for once this one's scores are there and its values once this one's are summed.  LDS only joins the waves: a row of V^T or K is read by one wave alone.
-// Bound by memory where the launch fills the chip: 32 sequences' next tokens, 64 heads on 8, up to 4096 positions in e4m3, 41 us (39 at a large copy's rate);
+// Bound by memory where the launch fills the chip: 32 sequences' next tokens, 64 heads on 8, up to 4096 positions in e4m3, 48 us (39 at a large copy's rate);
 // one behind 60001 positions of 32 heads in i8, 102 us (4.9 TB/s; at a copy's rate 108).  One behind 500 takes 11 us: two launches, and in each two or three trips
 // to memory that wait for one another.
 template <int KV, int NP, int D>
@@ -895,7 +895,8 @@ void kv_attention_plan(const KvLayer &l, int kv_type, const l2_kvbatch &b, const
         if (a.window) seen = std::min<int64_t>(seen, (int64_t)a.window + std::min(rows, per_tile) + a.sinks + 2 * tt);
         return (seen + tt - 1) / tt;
     };
-    // parts so that `full` blocks come to be, of `least` tiles or more
+    // Parts so that `full` blocks come to be, of `least` tiles or more.  Two narrow blocks per CU: with 3, 4 and 6 the step of 32 sequences above took 55, 52 and 56 us instead
+    // of 48.  One wide block, which fills a CU: three parts instead of one, of a batch of twelve, cost 28 us of joining and saved none.
     auto parts_of = [&](int64_t blocks, int64_t full, int64_t tiles, int64_t least, int *splits, int *per) {
         const int64_t parts = std::max<int64_t>(1, std::min<int64_t>((full + blocks - 1) / blocks, tiles / least));
         *per = (int)((tiles + parts - 1) / parts);
