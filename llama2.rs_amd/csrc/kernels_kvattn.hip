@@ -408,45 +408,70 @@ __device__ __forceinline__ float row_max(float v) { // of a row of 16 lanes: 1, 
 }
 __device__ __forceinline__ float wave_max(float v) { return lanes::rows_max(row_max(v)); }
 
-// Joins the parts of each query row: a block per row and head, its waves parts in turn.  NARROW: block x has row x % most of sequence x / most, most rows at the most;
-// else row x.
-constexpr int kJoinWaves = 4;
-template <int D, bool NARROW>
+// Joins the parts of each query row.  Of up to kFewParts parts (FEW) a wave has a row and head to itself, its lanes a part's statistics each; of more the four waves of a
+// block share one, parts in turn.  NARROW: block x has row x % most of sequence x / most, most rows at the most; else row x.
+constexpr int kJoinWaves = 4, kFewParts = 8;
+template <int D, bool NARROW, bool FEW>
 __global__ __launch_bounds__(64 * kJoinWaves) void kv_join_kernel(l2_kvbatch b, KvAttention a, Parts parts, int splits, int stride, int group, int most) {
-    const int hq = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hq = FEW ? kJoinWaves * blockIdx.y + w : blockIdx.y;
     const int i = NARROW ? (int)blockIdx.x / most : kv::sequence_of(b, blockIdx.x);
     if (i >= b.n_seqs) return;
     const kv::Seq s = kv::sequence(b, i);
     const int row = NARROW ? s.first + (int)blockIdx.x % most : blockIdx.x;
     if (row - s.first >= s.rows || (s.rows <= most) != NARROW) return;
+    if (FEW && hq >= a.n_heads) return;
     const int64_t at = ((int64_t)row * a.n_heads + hq) * stride;
-    __shared__ float sh_acc[kJoinWaves][D], sh_sum[kJoinWaves];
-    float o = -kInf;
-    for (int x = lane; x < splits; x += 64) o = fmaxf(o, parts.stat[at + x].x);
-    o = wave_max(o);
+    auto none = [](float2 st) { return st.y == 0.f && st.x == -kInf; }; // nothing of it is there
     constexpr int E = D / 64;
-    float v[E] = {}, total = 0.f;
+    float v[E] = {};
+    if constexpr (FEW) {
+        const float2 st = lane < splits ? parts.stat[at + lane] : make_float2(-kInf, 0.f);
+        float part[kFewParts][E] = {};
+#pragma unroll
+        for (int x = 0; x < kFewParts; x++)
+            if (x < splits)
+#pragma unroll
+                for (int e = 0; e < E; e++) part[x][e] = parts.acc[(at + x) * D + E * lane + e];
+        const float o = wave_max(st.x), f = none(st) ? 0.f : st.x == o ? 1.f : __builtin_amdgcn_exp2f(st.x - o), mine = none(st) ? 0.f : st.y * f;
+        const int is = !none(st);
+        float sum = 0.f;
+#pragma unroll
+        for (int x = 0; x < kFewParts; x++) {
+            const float fx = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), x));
+            sum += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), x));
+            if (__builtin_amdgcn_readlane(is, x))
+#pragma unroll
+                for (int e = 0; e < E; e++) v[e] += part[x][e] * fx;
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++) kv::store(a.out, a.type, row * a.out_stride + (int64_t)hq * D + E * lane + e, sum == 0.f ? 0.f : v[e] / sum);
+    } else {
+        __shared__ float sh_acc[kJoinWaves][D], sh_sum[kJoinWaves];
+        float o = -kInf;
+        for (int x = lane; x < splits; x += 64) o = fmaxf(o, parts.stat[at + x].x);
+        o = wave_max(o);
+        float total = 0.f;
 #pragma unroll 4
-    for (int x = w; x < splits; x += kJoinWaves) {
-        const float2 st = parts.stat[at + x];
-        float part[E];
+        for (int x = w; x < splits; x += kJoinWaves) {
+            const float2 st = parts.stat[at + x];
+            float part[E];
 #pragma unroll
-        for (int e = 0; e < E; e++) part[e] = parts.acc[(at + x) * D + E * lane + e];
-        const bool none = st.y == 0.f && st.x == -kInf; // nothing of it is there
-        const float f = none ? 0.f : st.x == o ? 1.f : __builtin_amdgcn_exp2f(st.x - o);
-        total += none ? 0.f : st.y * f;
+            for (int e = 0; e < E; e++) part[e] = parts.acc[(at + x) * D + E * lane + e];
+            const float f = none(st) ? 0.f : st.x == o ? 1.f : __builtin_amdgcn_exp2f(st.x - o);
+            total += none(st) ? 0.f : st.y * f;
 #pragma unroll
-        for (int e = 0; e < E; e++) v[e] += none ? 0.f : part[e] * f;
+            for (int e = 0; e < E; e++) v[e] += none(st) ? 0.f : part[e] * f;
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++) sh_acc[w][E * lane + e] = v[e];
+        if (lane == 0) sh_sum[w] = total;
+        __syncthreads();
+        if (threadIdx.x >= D) return;
+        float sum = 0.f, acc = 0.f;
+#pragma unroll
+        for (int x = 0; x < kJoinWaves; x++) sum += sh_sum[x], acc += sh_acc[x][threadIdx.x];
+        kv::store(a.out, a.type, row * a.out_stride + (int64_t)hq * D + threadIdx.x, sum == 0.f ? 0.f : acc / sum);
     }
-#pragma unroll
-    for (int e = 0; e < E; e++) sh_acc[w][E * lane + e] = v[e];
-    if (lane == 0) sh_sum[w] = total;
-    __syncthreads();
-    if (threadIdx.x >= D) return;
-    float sum = 0.f, acc = 0.f;
-#pragma unroll
-    for (int x = 0; x < kJoinWaves; x++) sum += sh_sum[x], acc += sh_acc[x][threadIdx.x];
-    kv::store(a.out, a.type, row * a.out_stride + (int64_t)hq * D + threadIdx.x, sum == 0.f ? 0.f : acc / sum);
 }
 
 typedef float f16v __attribute__((ext_vector_type(16)));
@@ -877,7 +902,8 @@ typedef void (*AttnKernel)(KvLayer, l2_kvbatch, KvAttention, Parts, Cut);
      {SIZES(kernel, 3, 1), SIZES(kernel, 3, 2), SIZES(kernel, 3, 3)}}
 const AttnKernel kNarrow[4][3][2] = ALL(kv_narrow_kernel), kWide[4][3][2] = ALL(kv_wide_kernel);
 typedef void (*JoinKernel)(l2_kvbatch, KvAttention, Parts, int, int, int, int);
-const JoinKernel kJoin[2][2] = {{kv_join_kernel<64, false>, kv_join_kernel<64, true>}, {kv_join_kernel<128, false>, kv_join_kernel<128, true>}};
+const JoinKernel kJoin[2][2][2] = {{{kv_join_kernel<64, false, false>, kv_join_kernel<64, false, true>}, {kv_join_kernel<64, true, false>, kv_join_kernel<64, true, true>}},
+                                   {{kv_join_kernel<128, false, false>, kv_join_kernel<128, false, true>}, {kv_join_kernel<128, true, false>, kv_join_kernel<128, true, true>}}};
 
 // In how many 16-bit numbers q and the weights enter the matrix cores, less one.
 int pieces_index(int kv_type, int type) {
@@ -903,8 +929,8 @@ void kv_attention_plan(const KvLayer &l, int kv_type, const l2_kvbatch &b, const
         *splits = *per ? (int)((tiles + *per - 1) / *per) : 1;
     };
     plan->wide = rows * group > kNarrowRows;
-    // A single sequence is the one kernel's or the other's; several may be some of each.
-    plan->narrow_rows = group > kNarrowRows || (plan->wide && seqs == 1) ? 0 : kNarrowRows / group * group;
+    // The one kernel's or the other's alone, where every sequence has that many rows if the call's arrays are full; else they may be some of each.
+    plan->narrow_rows = group > kNarrowRows || (plan->wide && (b.n_rows - (seqs - 1) * rows) * group > kNarrowRows) ? 0 : kNarrowRows / group * group;
     plan->narrow_splits = plan->wide_splits = 1;
     if (plan->narrow_rows)
         parts_of((plan->wide ? (seqs + 1) / 2 : seqs) * l.n_heads, 2 * cu_count(), tiles_seen(kv_type <= L2_KV_E4M3 ? 64 : 32, kNarrowRows), kNarrowWaves, &plan->narrow_splits,
@@ -935,11 +961,13 @@ int kv_attention_launch(const KvLayer &l, int kv_type, const l2_kvbatch &b, cons
         l2_launch(kNarrow[kv_type][np][big], dim3(plan.narrow_splits, l.n_heads, b.n_seqs), dim3(64 * kNarrowWaves), 0, st, l, b, a, parts,
                   Cut{plan.narrow_splits, plan.narrow_per, plan.stride, plan.narrow_rows});
     const int most = plan.narrow_rows / group; // rows of a sequence that the narrow kernel takes
-    if (plan.narrow_rows && plan.narrow_splits > 1)
-        l2_launch(kJoin[big][1], dim3(b.n_seqs * std::min(most, b.max_rows), a.n_heads), dim3(64 * kJoinWaves), 0, st, b, a, parts, plan.narrow_splits, plan.stride, group,
-                  std::min(most, b.max_rows));
-    if (plan.wide && plan.wide_splits > 1)
-        l2_launch(kJoin[big][0], dim3(b.n_rows, a.n_heads), dim3(64 * kJoinWaves), 0, st, b, a, parts, plan.wide_splits, plan.stride, group, most);
+    auto join = [&](bool narrow, int blocks, int splits, int most) {
+        const bool few = splits <= kFewParts;
+        l2_launch(kJoin[big][narrow][few], dim3(blocks, few ? (a.n_heads + kJoinWaves - 1) / kJoinWaves : a.n_heads), dim3(64 * kJoinWaves), 0, st, b, a, parts, splits,
+                  plan.stride, group, most);
+    };
+    if (plan.narrow_rows && plan.narrow_splits > 1) join(true, b.n_seqs * std::min(most, b.max_rows), plan.narrow_splits, std::min(most, b.max_rows));
+    if (plan.wide && plan.wide_splits > 1) join(false, b.n_rows, plan.wide_splits, most);
     L2_HIP(hipGetLastError());
     return L2_OK;
 }
@@ -951,6 +979,8 @@ int kv_attention_warm_up() {
             for (auto &n : k)
                 for (AttnKernel f : n)
                     if (f) L2_HIP(hipFuncGetAttributes(&a, (const void *)f));
-    for (auto &k : kJoin) for (JoinKernel f : k) L2_HIP(hipFuncGetAttributes(&a, (const void *)f));
+    for (auto &d : kJoin)
+        for (auto &k : d)
+            for (JoinKernel f : k) L2_HIP(hipFuncGetAttributes(&a, (const void *)f));
     return L2_OK;
 }
