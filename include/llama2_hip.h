@@ -257,9 +257,9 @@ typedef struct l2_kvbatch {
     const int32_t *pages;   /* [n_seqs][max_pages] */
     int32_t n_seqs;         /* up to 65535 */
     int32_t max_pages;
-    int32_t n_rows;     /* rows of the call's arrays */
+    int32_t n_rows;     /* rows of the call's arrays, up to 2^22 (times the query heads of a kv head, 2^30) */
     int32_t max_rows;   /* the most rows of a sequence */
-    int32_t max_length; /* the most positions of a sequence */
+    int32_t max_length; /* the most positions of a sequence, up to 2^30 */
 } l2_kvbatch;
 
 /* Writes rows into one layer: k_dev and v_dev of `type`, [n_rows][n_kv_heads][head_size] with k_stride and v_stride elements from row to

@@ -115,6 +115,7 @@ static int check_batch(const l2_kvpool *p, const l2_kvbatch *b) {
         return l2_fail(L2_ERR_ARG, "batch of %d sequences (up to 65535), %d rows, limits %d pages, %d rows, %d positions", b->n_seqs, b->n_rows, b->max_pages,
                        b->max_rows, b->max_length);
     if (b->n_rows > 1 << 22) return l2_fail(L2_ERR_RANGE, "%d rows (up to 2^22)", b->n_rows);
+    if (b->max_length > 1 << 30) return l2_fail(L2_ERR_RANGE, "%d positions (up to 2^30)", b->max_length);
     if ((int64_t)b->max_length > (int64_t)b->max_pages * p->page_size)
         return l2_fail(L2_ERR_ARG, "%d positions do not fit %d pages of %d", b->max_length, b->max_pages, p->page_size);
     if (b->n_seqs && (!b->starts || !b->lengths || (b->max_pages && !b->pages))) return l2_fail(L2_ERR_ARG, "null argument");
@@ -159,6 +160,8 @@ static int check_attention(const l2_kvpool *p, const l2_kvbatch *batch, const l2
     L2_TRY(check_type(a->type));
     if (a->n_heads < 1 || a->n_heads > 65535 || a->n_heads % p->n_kv_heads)
         return l2_fail(L2_ERR_ARG, "%d query heads over %d kv heads", a->n_heads, p->n_kv_heads);
+    if ((int64_t)batch->n_rows * (a->n_heads / p->n_kv_heads) > 1 << 30)
+        return l2_fail(L2_ERR_RANGE, "%d rows of %d query heads to a kv head (up to 2^30 together)", batch->n_rows, a->n_heads / p->n_kv_heads);
     if (!(a->scale >= 0.f && a->scale < INFINITY)) return l2_fail(L2_ERR_ARG, "scale %g", (double)a->scale);
     if (a->window < 0 || a->sinks < 0) return l2_fail(L2_ERR_ARG, "window %d, sinks %d", a->window, a->sinks);
     *out = KvAttention{};

@@ -141,6 +141,13 @@ static void calls(int kv_type) {
     l2_kvbatch many = good;
     many.n_rows = (1 << 22) + 1;
     REFUSED(L2_ERR_RANGE, write(&many));
+    many = good;
+    many.max_pages = 1 << 26, many.max_length = (1 << 30) + 1;
+    REFUSED(L2_ERR_RANGE, write(&many));
+    many = good;
+    many.n_rows = 1 << 22;
+    const l2_attention wide{257 * heads, L2_F32, 0.f, 0, 0, 0, 0};
+    REFUSED(L2_ERR_RANGE, l2_kvpool_attention(p, 0, &many, &wide, (void *)64, (void *)128, (void *)64, 1000, st));
     REFUSED(L2_ERR_ARG, write(nullptr));
     REFUSED(L2_ERR_ARG, l2_kvpool_write(nullptr, 0, &good, (void *)64, (void *)64, L2_F32, 0, 0, st));
     // layers, types, addresses, strides
