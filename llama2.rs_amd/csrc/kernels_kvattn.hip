@@ -517,8 +517,8 @@ __device__ __forceinline__ void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n
 //
 // Of heads of 128, a wave's products of a tile are 1024 clocks of its matrix core, per number that q and p are made of.  A step is about 2000 of 16-bit cells, where
 // the exponentials and the loads' issue are as long as the products and theirs, and 2600 of 8-bit ones, where the vector ALUs are busy throughout: each score and
-// weight is multiplied by a scale, and conversion is theirs too.  512 rows of 64 heads on 8 behind 7488 positions in i8: 180 us, 720 TFLOP/s (a large library product in
-// fp16: 1170); two prompts of 4096 and 2542, 32 heads, window 1024, bf16: 168 us, 560 TFLOP/s.  What did not pay: one conversion spread between the products
+// weight is multiplied by a scale, and conversion is theirs too.  512 rows of 64 heads on 8 behind 7488 positions in i8: 169 us, 770 TFLOP/s (a large library product in
+// fp16: 1170); two prompts of 4096 and 2542, 32 heads, window 1024, bf16: 166 us, 570 TFLOP/s, of which a quarter is the last of four rounds of blocks.  What did not pay: one conversion spread between the products
 // (+9 %), the values' wait half a tile later, scales as float4 from LDS (16 reads a tile; they now are two registers, broadcast in rows of lanes).
 template <int KV, int NP, int D>
 __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, Cut cut) {
