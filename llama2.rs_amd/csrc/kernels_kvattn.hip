@@ -147,7 +147,7 @@ struct Parts {
     float2 *stat; // [row][head][split]: off, sum
 };
 
-// Sequences of up to 16 query rows per kv head (new tokens x query heads of the group).  A block has one sequence, kv head and part of the positions, its
+// Sequences of few query rows per kv head (new tokens x query heads of the group).  A block has 16 rows of one sequence and kv head and part of the positions, its
 // four waves tiles of 64 positions (32 of 16-bit cells) in turn, straight from memory into registers: 8 KB of keys and 8 KB of values, the next tile's keys
 // asked for once this one's scores are there and its values once this one's are summed.  LDS only joins the waves: a row of V^T or K is read by one wave alone.
 // Bound by memory where the launch fills the chip: 32 sequences' next tokens, 64 heads on 8, up to 4096 positions in e4m3, 48 us (39 at a large copy's rate);
@@ -158,15 +158,15 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
     using C = Cells<KV>;
     using Frag = typename C::Frag;
     constexpr int TT = 64 / C::kSize, ST = TT / 16, CH = TT / 4, FR = 2 / C::kSize, KL = D * C::kSize / 64, DT = D / 16, VS = TT / 32;
-    const int split = blockIdx.x, h = blockIdx.y, i = blockIdx.z;
+    const int split = blockIdx.x % cut.splits, r0 = kNarrowRows * (blockIdx.x / cut.splits), h = blockIdx.y, i = blockIdx.z;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
     const kv::Seq s = kv::sequence(b, i);
     const int group = a.n_heads / l.n_heads, rows = s.rows * group;
-    if (rows == 0 || rows > cut.narrow) return;
+    if (r0 >= rows || rows > cut.narrow) return;
     const int base = s.length - s.rows; // position of the first row
-    const bool real = m < rows;
-    const Seen seen(a, real ? base + m / group : -1);
-    const int64_t q_row = s.first + (real ? m / group : 0), head = h * group + (real ? m % group : 0);
+    const bool real = r0 + m < rows;
+    const Seen seen(a, real ? base + (r0 + m) / group : -1);
+    const int64_t q_row = s.first + (real ? (r0 + m) / group : 0), head = h * group + (real ? (r0 + m) % group : 0);
 
     const Range range = range_of<TT>(a, base, s.length - 1);
     const int begin = min(split * cut.per, range.n), end = min(begin + cut.per, range.n);
@@ -358,7 +358,7 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
     for (int x = 0; x < DT; x++) *(f4 *)&sh_acc[w][m][16 * x + 4 * g] = acc[x];
     if (g == 0) sh_stat[w][m] = make_float2(off, sum);
     __syncthreads();
-    for (int x = threadIdx.x; x < rows * (D / 4); x += 64 * kNarrowWaves) {
+    for (int x = threadIdx.x; x < min(rows - r0, kNarrowRows) * (D / 4); x += 64 * kNarrowWaves) {
         const int r = x / (D / 4), d = 4 * (x % (D / 4));
         float o = -kInf, total = 0.f;
 #pragma unroll
@@ -372,7 +372,7 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
             total += st.y * f;
             v += *(const f4 *)&sh_acc[y][r][d] * f;
         }
-        const int64_t row = s.first + r / group, hq = h * group + r % group;
+        const int64_t row = s.first + (r0 + r) / group, hq = h * group + (r0 + r) % group;
         if (cut.splits == 1) {
             const float inv = total == 0.f ? 0.f : 1.f / total;
             for (int j = 0; j < 4; j++) v[j] = total == 0.f ? 0.f : v[j] * inv;
@@ -928,13 +928,19 @@ void kv_attention_plan(const KvLayer &l, int kv_type, const l2_kvbatch &b, const
         *per = (int)((tiles + parts - 1) / parts);
         *splits = *per ? (int)((tiles + *per - 1) / *per) : 1;
     };
-    plan->wide = rows * group > kNarrowRows;
+    // Where no sequence has more than `most` rows the narrow kernel takes all, cells read once for each 16 rows.  us as narrow and wide, 32 sequences of 2048 positions, 64 heads on
+    // 8: 24, 48 and 64 rows of bf16 on e4m3 53 / 101, 76 / 104 and 88 / 104 (80: 112 / 108), of fp32 on i8 57 / 142, 82 / 148 and 98 / 150, of fp32 on bf16 103 / 260, 138 / 260 and
+    // 167 / 258; of fp16 on fp16, where a block's cells are twice as many and the wide kernel has the least to do, 100 / 104 (32: 101 / 105), 131 / 109 and 173 / 112.
+    const int most = (kv_type > L2_KV_E4M3 && pieces_index(kv_type, a.type) == 0 ? 32 : 64) / group * group;
+    plan->wide = rows * group > most;
     // The one kernel's or the other's alone, where every sequence has that many rows if the call's arrays are full; else they may be some of each.
-    plan->narrow_rows = group > kNarrowRows || (plan->wide && (b.n_rows - (seqs - 1) * rows) * group > kNarrowRows) ? 0 : kNarrowRows / group * group;
+    if (!plan->wide) plan->narrow_rows = most;
+    else plan->narrow_rows = group > kNarrowRows || (b.n_rows - (seqs - 1) * rows) * group > kNarrowRows ? 0 : kNarrowRows / group * group;
+    plan->narrow_blocks = (int)std::max<int64_t>((std::min<int64_t>(rows * group, plan->narrow_rows) + kNarrowRows - 1) / kNarrowRows, 1);
     plan->narrow_splits = plan->wide_splits = 1;
     if (plan->narrow_rows)
-        parts_of((plan->wide ? (seqs + 1) / 2 : seqs) * l.n_heads, 2 * cu_count(), tiles_seen(kv_type <= L2_KV_E4M3 ? 64 : 32, kNarrowRows), kNarrowWaves, &plan->narrow_splits,
-                 &plan->narrow_per);
+        parts_of((plan->wide ? (seqs + 1) / 2 : seqs) * l.n_heads * plan->narrow_blocks, 2 * cu_count(), tiles_seen(kv_type <= L2_KV_E4M3 ? 64 : 32, plan->narrow_rows),
+                 kNarrowWaves, &plan->narrow_splits, &plan->narrow_per);
     // row tiles of all sequences, at most: their whole ones, and a last one of each that has more rows than the narrow kernel takes
     const int64_t all = (int64_t)b.n_rows * group;
     const int64_t tile = kWideRows;
@@ -958,7 +964,7 @@ int kv_attention_launch(const KvLayer &l, int kv_type, const l2_kvbatch &b, cons
                   Cut{plan.wide_splits, plan.wide_per, plan.stride, plan.narrow_rows});
     }
     if (plan.narrow_rows)
-        l2_launch(kNarrow[kv_type][np][big], dim3(plan.narrow_splits, l.n_heads, b.n_seqs), dim3(64 * kNarrowWaves), 0, st, l, b, a, parts,
+        l2_launch(kNarrow[kv_type][np][big], dim3(plan.narrow_splits * plan.narrow_blocks, l.n_heads, b.n_seqs), dim3(64 * kNarrowWaves), 0, st, l, b, a, parts,
                   Cut{plan.narrow_splits, plan.narrow_per, plan.stride, plan.narrow_rows});
     const int most = plan.narrow_rows / group; // rows of a sequence that the narrow kernel takes
     auto join = [&](bool narrow, int blocks, int splits, int most) {

@@ -39,6 +39,7 @@ struct KvAttnPlan {
     size_t workspace;               // bytes
     bool wide;                      // whether there may be sequences of more rows than ..
     int narrow_rows;                // .. the narrow kernel takes, per kv head; 0: it takes none
+    int narrow_blocks;              // of 16 rows, of a sequence and kv head
     int narrow_splits, wide_splits; // parts that positions are cut into,
     int narrow_per, wide_per;       // each of so many tiles
     int stride;                     // the larger of both: parts of a row in the workspace

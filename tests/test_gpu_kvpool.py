@@ -215,6 +215,20 @@ def test_long_contexts(dev, kv, t):
     c.close()
 
 
+@pytest.mark.parametrize("kv,t", [("i8", F16), ("i8", F32), ("e4m3", BF16), ("f16", F16), ("f16", F32), ("bf16", BF16), ("bf16", F32)])
+@pytest.mark.parametrize("group,most", [(1, 64), (5, 12), (8, 4), (8, 9), (32, 1), (40, 1), (72, 1)])
+def test_a_few_tokens_each(dev, kv, t, group, most):
+    """Up to 17, 32, 64 and some more query rows per kv head, which are blocks of 16, of one kernel or the other."""
+    rows = [most, 1, (most + 1) // 2, most, 0]
+    lengths = [most, 500, 333, 70, 20]
+    c, rng = _filled(dev, kv, 16, 2, 64 if group == 5 else 128, lengths, seed=group, t=t)
+    q = rng.standard_normal((sum(rows) + 3, 2 * group, c.head_size)).astype(np.float32)
+    for window, sinks in ((0, 0), (90, 5)):
+        got = c.attend(q, None, t, 2 * group, window, sinks, batch=c.batch(rows, first=1, behind=2))
+        c.check(got, q, rows, t, 2 * group, window, sinks, first=1)
+    c.close()
+
+
 @pytest.mark.parametrize("kv,t", [("i8", F16), ("e4m3", F32), ("f16", BF16), ("bf16", F32)])
 def test_groups_that_do_not_divide_a_tile(dev, kv, t):
     """Chunks of several tiles of rows whose borders lie inside a token's heads, behind many tiles that all of them see."""
