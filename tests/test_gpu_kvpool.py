@@ -510,6 +510,26 @@ def test_results_do_not_depend_on_the_batch_or_the_run(dev):
     c.close()
 
 
+def test_a_workspace_for_any_limits(dev):
+    """The smallest, the largest and any limits between have a plan; empty calls want no workspace and do nothing."""
+    from llama2_rs import ops
+    rng = np.random.default_rng(12)
+    pools = [ops.KvPool(1, 4, 64, heads, d, kv) for heads, d, kv in ((1, 64, "i8"), (8, 128, "bf16"))]
+    ends = [0, 1, 2, 3, 16, 17, 64, 65, 255, 256, 257, 4096]
+    any_of = lambda most: int(rng.choice(ends + [most])) if rng.random() < 0.7 else int(2 ** rng.uniform(0, np.log2(most)))  # noqa: E731
+    for n in range(4000):
+        p = pools[n % 2]
+        seqs, rows, most, length = min(any_of(65535), 65535), min(any_of(1 << 22), 1 << 22), any_of(1 << 22), any_of(1 << 30)
+        group = int(rng.choice([1, 2, 3, 8, 16, 17, 33, 64, 65, 255]))
+        b = ops.KvBatch(64, 64, 64, seqs, -(-length // 64), rows, most, length)
+        need = p.attention_workspace(b, group * (8 if n % 2 else 1), int(rng.integers(3)), int(rng.choice([0, 1, 100, 2 ** 31 - 1])), int(rng.choice([0, 5, 2 ** 31 - 1])))
+        assert 0 <= need < 2 ** 62
+        if seqs == 0 or rows == 0 or most == 0:
+            p.attention(0, b, 0, 0, group * (8 if n % 2 else 1))
+    for p in pools:
+        p.close()
+
+
 def test_contents_beyond_the_limits_touch_nothing_else(dev):
     """Arrays that say more than the call's limits: nothing outside of the rows and the pool's own pages is written."""
     c, rng = _filled(dev, "i8", 16, 1, 64, [64, 64])
