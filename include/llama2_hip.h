@@ -276,8 +276,8 @@ int l2_kvpool_read(l2_kvpool *p, int layer, const l2_kvbatch *batch, void *k_dev
  * head h reads kv head h / (n_heads / n_kv_heads)); out may be q, with its stride.  The row of position pos sees the positions t <= pos that have a page, with a window > 0
  * only those of the last `window` (t > pos - window) and of the first `sinks`.  out = sum over t of softmax(scale * q.k_t) v_t;
  * zeros where nothing is seen.  Keys and values come from the pool, those of the rows included (l2_kvpool_write first).  Scores, statistics and sums
- * are fp32; q and the softmax's weights enter the matrix cores as one 16-bit number each for 16-bit rows and as several, to within 2^-22,
- * for fp32 rows.  What is not seen has no influence, NaN and infinities included. */
+ * are fp32; q of 16 bits enters the matrix cores as it is, fp32 q and all weights of the softmax as several 16-bit numbers: to within 2^-22
+ * (over L2_KV_BF16 2^-24, for 16-bit rows 2^-16).  What is not seen has no influence, NaN and infinities included. */
 typedef struct l2_attention {
     int32_t n_heads;
     int32_t type;       /* L2_F32, L2_F16 or L2_BF16 */

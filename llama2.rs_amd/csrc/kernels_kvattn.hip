@@ -8,8 +8,10 @@
 // Weights enter the second product in 16 bits, times a factor that cancels in the quotient with their sum: p_t = exp2(s_t - off).  `off` follows the tiles' max s + e, where
 // 2^e is the power of two above the largest scale of their values, so that p_t * (scale of v_t) is what is bounded, by 2^15 for fp16: off goes to 7 below max s + e, and
 // is left where it is until that lies more than 8 higher, so that sums are seldom rescaled (a tile of 32 rows would have a new maximum among them nearly always).
-// fp32 rows have q and p in two fp16 numbers (2^-22; a weight that is 2^-21 of the largest or less, to within 2^-32 of the largest) or, over a pool in
-// bf16, in three; rows of 16 bits in one where that holds a q as it is.  q is scaled by a power of two per row, so that fp16 holds what bf16 and fp32 rows may contain.
+// Weights are two fp16 numbers each (to within 2^-22, and no less than 2^-32 of the largest) or, over a pool in bf16, two of bf16 (2^-16) for rows of 16 bits and three for
+// fp32 rows.  One would be what a result's own rounding is: of rows in fp16 and bf16 over pools in i8 and bf16 they then were off by 1.4 and 1.3 times what fp32 weights leave, 2.9e-4 for
+// 2.1e-4 and 2.1e-3 for 1.6e-3.  q is one number where that holds it as it is, as many as a weight for fp32 rows, two for fp16 rows over bf16; for fp16 numbers scaled by a power of two per
+// row, so that they hold what bf16 and fp32 rows may contain.
 #include <algorithm>
 
 #include "kvpool.h"
@@ -76,23 +78,23 @@ struct Cells {
 __device__ __forceinline__ f4 mfma16(const h8 &a, const h8 &b, const f4 &c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f4 mfma16(const b8 &a, const b8 &b, const f4 &c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
-// x as a sum of NP numbers of 16 bits, each the nearest to what those before it leave.  The compiler may make a product and its rounding to fp16
-// one instruction that rounds once, for one of the two places that the first number goes to: x is a value that it knows nothing of.
+// x as a sum of NP numbers of 16 bits, each the nearest to what those before it leave.  Two at a time, as one instruction converts them and takes the numbers out of its
+// result again; that is a value which the compiler knows nothing of, so that it cannot make a product and its rounding one operation for one of the two places it goes to.
 template <class Frag, class One, int NP>
 __device__ __forceinline__ void pieces(f8 x, Frag (&out)[NP]) {
-    if (NP > 1)
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            float v = x[j];
-            asm("" : "+v"(v));
-            x[j] = v;
-        }
+    typedef One two __attribute__((ext_vector_type(2)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    float minus = -1.f; // unknown too: a product with a number of 16 bits and a sum are one instruction, a difference from one is two
+    if (NP > 1) asm("" : "+s"(minus));
 #pragma unroll
     for (int i = 0; i < NP; i++) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            out[i][j] = (One)x[j];
-            if (i + 1 < NP) x[j] -= (float)out[i][j];
+        for (int j = 0; j < 8; j += 2) {
+            uint32_t bits = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{x[j], x[j + 1]}, two));
+            if (i + 1 < NP) asm("" : "+v"(bits));
+            const two n = __builtin_bit_cast(two, bits);
+            out[i][j] = n[0], out[i][j + 1] = n[1];
+            if (i + 1 < NP) x[j] = fmaf((float)n[0], minus, x[j]), x[j + 1] = fmaf((float)n[1], minus, x[j + 1]);
         }
     }
 }
@@ -135,6 +137,9 @@ __device__ __forceinline__ u4 finite(u4 v, bool &odd) {
 
 constexpr int kNarrowRows = 16, kNarrowWaves = 4;
 
+// The numbers that a weight is, of rows whose q is NQ.
+constexpr int weight_numbers(int nq) { return nq == 3 ? 3 : 2; }
+
 // How a launch cuts positions: `splits` parts of `per` tiles each, `stride` parts of a row in the workspace; and the query rows per kv head of a sequence up to which
 // it is the narrow kernel's.
 struct Cut {
@@ -153,11 +158,11 @@ struct Parts {
 // Bound by memory where the launch fills the chip: 32 sequences' next tokens, 64 heads on 8, up to 4096 positions in e4m3, 48 us (39 at a large copy's rate);
 // one behind 60001 positions of 32 heads in i8, 102 us (4.9 TB/s; at a copy's rate 108).  One behind 500 takes 11 us: two launches, and in each two or three trips
 // to memory that wait for one another.
-template <int KV, int NP, int D>
+template <int KV, int NQ, int D>
 __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, Cut cut) {
     using C = Cells<KV>;
     using Frag = typename C::Frag;
-    constexpr int TT = 64 / C::kSize, ST = TT / 16, CH = TT / 4, FR = 2 / C::kSize, KL = D * C::kSize / 64, DT = D / 16, VS = TT / 32;
+    constexpr int TT = 64 / C::kSize, ST = TT / 16, CH = TT / 4, FR = 2 / C::kSize, KL = D * C::kSize / 64, DT = D / 16, VS = TT / 32, NP = weight_numbers(NQ);
     const int split = blockIdx.x % cut.splits, r0 = kNarrowRows * (blockIdx.x / cut.splits), h = blockIdx.y, i = blockIdx.z;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
     const kv::Seq s = kv::sequence(b, i);
@@ -224,7 +229,7 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
         if (n + kNarrowWaves < end) pages(n + kNarrowWaves);
     }
     // q: this lane's row, the dimensions that lie across from its 16 bytes of a key
-    Frag q[D / 32][NP];
+    Frag q[D / 32][NQ];
     float c; // exponent of two per unit of the scores' sums
     {
         f8 x[D / 32];
@@ -246,7 +251,7 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
             c = ldexpf(c, -e);
         }
 #pragma unroll
-        for (int k = 0; k < D / 32; k++) pieces<Frag, typename C::One, NP>(x[k], q[k]);
+        for (int k = 0; k < D / 32; k++) pieces<Frag, typename C::One, NQ>(x[k], q[k]);
     }
 
     f4 acc[DT] = {};
@@ -261,7 +266,7 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
             for (int x = 0; x < ST; x++) {
                 const Frag f = C::frag(kr[x][k / FR], k % FR);
 #pragma unroll
-                for (int y = 0; y < NP; y++) sc[x] = mfma16(f, q[k][y], sc[x]);
+                for (int y = 0; y < NQ; y++) sc[x] = mfma16(f, q[k][y], sc[x]);
             }
         if (C::kEight)
 #pragma unroll
@@ -515,16 +520,16 @@ __device__ __forceinline__ void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n
 // and its exponentials in 2 i + 1, the others each a step later.  So keys of tile i are read in steps 2 i and 2 i + 1, its values in 2 i + 2 and 2 i + 3, its scales in 2 i + 1 and 2 i + 2;
 // with two places for keys and three for the rest, tile i + 1 may be written from step 2 i on, and is there before 2 i + 2.
 //
-// Of heads of 128, a wave's products of a tile are 1024 clocks of its matrix core, per number that q and p are made of.  A step is about 2000 of 16-bit cells, where
-// the exponentials and the loads' issue are as long as the products and theirs, and 2600 of 8-bit ones, where the vector ALUs are busy throughout: each score and
-// weight is multiplied by a scale, and conversion is theirs too.  512 rows of 64 heads on 8 behind 7488 positions in i8: 169 us, 770 TFLOP/s (a large library product in
-// fp16: 1170); two prompts of 4096 and 2542, 32 heads, window 1024, bf16: 166 us, 570 TFLOP/s, of which a quarter is the last of four rounds of blocks.  What did not pay: one conversion spread between the products
+// Of heads of 128, a wave's products of a tile are 512 clocks of its matrix core per number that q is made of, and as many per number of a weight: 1536 of 16-bit rows.  Each score
+// and weight of 8-bit cells is multiplied by a scale, and conversion is the vector ALUs' too.  512 rows of 64 heads on 8 behind 7488 positions in i8: 210 us, 620 TFLOP/s of what
+// one number each would take (a large library product in fp16: 1170); two prompts of 4096 and 2542, 32 heads, window 1024, bf16: 193 us, 490 TFLOP/s, of which a quarter is the last of four rounds of
+// blocks.  Weights in one number took 168 and 162.  What did not pay: one conversion spread between the products
 // (+9 %), the values' wait half a tile later, scales as float4 from LDS (16 reads a tile; they now are two registers, broadcast in rows of lanes).
-template <int KV, int NP, int D>
+template <int KV, int NQ, int D>
 __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, Cut cut) {
     using C = Cells<KV>;
     using Frag = typename C::Frag;
-    constexpr int TT = 64, PK = D / 8, DT = D / 32, KS = D / 16, LOADS = D * C::kSize / 64; // (of 16 bytes per lane: 16 positions)
+    constexpr int TT = 64, PK = D / 8, DT = D / 32, KS = D / 16, NP = weight_numbers(NQ), LOADS = D * C::kSize / 64; // (of 16 bytes per lane: 16 positions)
     __shared__ __align__(16) u4 sh_k[2][TT * PK], sh_v[3][D * 8];
     __shared__ __align__(16) float sh_ks[3][TT], sh_vs[3][TT];
     __shared__ __align__(16) float sh_top[3][4];
@@ -572,7 +577,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
     const int b_first = __builtin_amdgcn_readfirstlane(base + tile * kWideRows / group);
     const int b_last = __builtin_amdgcn_readfirstlane(base + (min((tile + 1) * kWideRows, rows) - 1) / group);
 
-    Frag q[KS][NP];
+    Frag q[KS][NQ];
     float c = a.scale * kLog2e;
     {
         kv::raw8 raw[KS];
@@ -598,7 +603,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
             if (C::kHalf)
 #pragma unroll
                 for (int j = 0; j < 8; j++) x[j] = ldexpf(x[j], e);
-            pieces<Frag, typename C::One, NP>(x, q[k]);
+            pieces<Frag, typename C::One, NQ>(x, q[k]);
         }
     }
 
@@ -702,7 +707,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
     // The weighted sum of one tile and the scores of the other, 2 x 32 positions.  Each of these products wants 16 bytes of LDS per lane, as long on their way as four
     // products take and no less of LDS's time than of the matrix cores': they are asked for kDeep products ahead.
     auto products = [&](auto with_values, auto with_scores, int vb, int kb) {
-        constexpr int V = decltype(with_values)::value ? 4 * DT : 0, K = decltype(with_scores)::value ? 2 * KS : 0, kDeep = NP == 1 ? 6 : 5 - NP;
+        constexpr int V = decltype(with_values)::value ? 4 * DT : 0, K = decltype(with_scores)::value ? 2 * KS : 0, kDeep = NQ == 1 ? 4 : 5 - NP;
         auto at = [&](int z) { return z < V ? v_at(vb, z % DT, z / DT) : k_at(kb, (z - V) / 2, (z - V) % 2); };
         if (K) sc[0] = sc[1] = f16v{};
         u4 ring[kDeep];
@@ -712,16 +717,19 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
         for (int z = 0; z < V + K; z++) {
             const Frag f = __builtin_bit_cast(Frag, ring[z % kDeep]);
             if (z + kDeep < V + K) ring[z % kDeep] = at(z + kDeep);
+            if (z < V) {
 #pragma unroll
-            for (int y = 0; y < NP; y++) {
-                if (z < V) acc[z % DT] = mfma32(f, pf[z / DT][y], acc[z % DT]);
-                else sc[(z - V) % 2] = mfma32(f, q[(z - V) / 2][y], sc[(z - V) % 2]);
+                for (int y = 0; y < NP; y++) acc[z % DT] = mfma32(f, pf[z / DT][y], acc[z % DT]);
+            } else {
+#pragma unroll
+                for (int y = 0; y < NQ; y++) sc[(z - V) % 2] = mfma32(f, q[(z - V) / 2][y], sc[(z - V) % 2]);
             }
         }
         __builtin_amdgcn_sched_group_barrier(0x100, kDeep, 0);
 #pragma unroll
         for (int z = 0; z < V + K; z++) {
-            __builtin_amdgcn_sched_group_barrier(0x8, NP, 0);
+            if (z < V) __builtin_amdgcn_sched_group_barrier(0x8, NP, 0);
+            else __builtin_amdgcn_sched_group_barrier(0x8, NQ, 0);
             if (z + kDeep < V + K) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
     };
@@ -757,9 +765,13 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
                 const int t = run_of(z) + 8 * hh;
                 const float v_scale = C::kEight ? scale_at<at % 16>(vs[at / 16]) : 0.f; // (by all lanes of the row)
                 const bool here = bits_there >> 8 * (2 * (z / 4) + (z / 2 & 1)) & 1, see = here & seen(t0 + t + r); // run t / 16
-                sc[z / 4][4 * (z & 3) + r] = see ? sc[z / 4][4 * (z & 3) + r] : -kInf;
+                const float score = sc[z / 4][4 * (z & 3) + r];
+                sc[z / 4][4 * (z & 3) + r] = see ? C::kEight ? fmaf(v_scale, 0.f, score) : score : -kInf; // NaN where the values are
                 if constexpr (C::kEight) top_v = fmaxf(top_v, see ? v_scale : 0.f);
             });
+            if (C::kEight)
+#pragma unroll
+                for (int z = 0; z < 2; z++) vs[z] = vs[z] == vs[z] ? vs[z] : 0.f; // nothing of a row that is not seen
             if (C::kEight) {
                 const lanes::Both v2 = lanes::both32(top_v);
                 top_v = fmaxf(v2.lo, v2.hi);
@@ -787,19 +799,9 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
                 p[j] = __builtin_amdgcn_exp2f(fmaf(sc[v / 2][8 * (v & 1) + j], c, -now));
                 sum += p[j];
             }
-            if constexpr (C::kEight) {
-                each<8>([&](auto j) { p[(int)j] *= scale_at<8 * (v & 1) + j>(vs[v / 2]); });
-                if (NP > 1 && !whole) // the scale of a row that is not seen may be NaN
-#pragma unroll
-                    for (int j = 0; j < 8; j++) p[j] = sc[v / 2][8 * (v & 1) + j] == -kInf ? 0.f : p[j];
-            }
+            if constexpr (C::kEight) each<8>([&](auto j) { p[(int)j] *= scale_at<8 * (v & 1) + j>(vs[v / 2]); });
             pieces<Frag, typename C::One, NP>(p, pf[v]);
         });
-        if (C::kEight && NP == 1 && !whole) // as above, but behind the loop, which then is a single run of instructions (more pieces leave no registers for it)
-#pragma unroll
-            for (int v = 0; v < 4; v++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) pf[v][0][j] = sc[v / 2][8 * (v & 1) + j] == -kInf ? (typename C::One)0.f : pf[v][0][j];
         // here, not where the compiler would have them: between the products, which then wait for the first ones
 #pragma unroll
         for (int v = 0; v < 4; v++)
@@ -896,7 +898,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
 }
 
 typedef void (*AttnKernel)(KvLayer, l2_kvbatch, KvAttention, Parts, Cut);
-#define SIZES(kernel, kv, np) {kernel<kv, np, 64>, kernel<kv, np, 128>}
+#define SIZES(kernel, kv, nq) {kernel<kv, nq, 64>, kernel<kv, nq, 128>}
 #define ALL(kernel)                                                                                                                             \
     {{SIZES(kernel, 0, 1), SIZES(kernel, 0, 2), {}}, {SIZES(kernel, 1, 1), SIZES(kernel, 1, 2), {}}, {SIZES(kernel, 2, 1), SIZES(kernel, 2, 2), {}}, \
      {SIZES(kernel, 3, 1), SIZES(kernel, 3, 2), SIZES(kernel, 3, 3)}}
@@ -905,7 +907,7 @@ typedef void (*JoinKernel)(l2_kvbatch, KvAttention, Parts, int, int, int, int);
 const JoinKernel kJoin[2][2][2] = {{{kv_join_kernel<64, false, false>, kv_join_kernel<64, false, true>}, {kv_join_kernel<64, true, false>, kv_join_kernel<64, true, true>}},
                                    {{kv_join_kernel<128, false, false>, kv_join_kernel<128, false, true>}, {kv_join_kernel<128, true, false>, kv_join_kernel<128, true, true>}}};
 
-// In how many 16-bit numbers q and the weights enter the matrix cores, less one.
+// In how many 16-bit numbers q enters the matrix cores, less one.
 int pieces_index(int kv_type, int type) {
     if (kv_type == L2_KV_BF16) return type == L2_BF16 ? 0 : type == L2_F16 ? 1 : 2;
     return type == L2_F32 ? 1 : 0;
@@ -954,17 +956,17 @@ void kv_attention_plan(const KvLayer &l, int kv_type, const l2_kvbatch &b, const
 
 int kv_attention_launch(const KvLayer &l, int kv_type, const l2_kvbatch &b, const KvAttention &a, const KvAttnPlan &plan, void *workspace, hipStream_t st) {
     if (b.n_rows == 0 || b.n_seqs == 0 || b.max_rows == 0) return L2_OK;
-    const int big = l.head_size == 128, group = a.n_heads / l.n_heads, np = pieces_index(kv_type, a.type);
+    const int big = l.head_size == 128, group = a.n_heads / l.n_heads, nq = pieces_index(kv_type, a.type);
     Parts parts{(float *)workspace, nullptr};
     parts.stat = (float2 *)(parts.acc + (size_t)b.n_rows * a.n_heads * plan.stride * l.head_size);
     if (plan.wide && plan.wide_tiles) {
         const int64_t blocks = plan.wide_tiles * l.n_heads * plan.wide_splits;
         if (blocks >= (int64_t)1 << 31) return l2_fail(L2_ERR_RANGE, "%d rows of %d heads", b.n_rows, a.n_heads);
-        l2_launch(kWide[kv_type][np][big], dim3((unsigned)blocks), dim3(kWideThreads), 0, st, l, b, a, parts,
+        l2_launch(kWide[kv_type][nq][big], dim3((unsigned)blocks), dim3(kWideThreads), 0, st, l, b, a, parts,
                   Cut{plan.wide_splits, plan.wide_per, plan.stride, plan.narrow_rows});
     }
     if (plan.narrow_rows)
-        l2_launch(kNarrow[kv_type][np][big], dim3(plan.narrow_splits * plan.narrow_blocks, l.n_heads, b.n_seqs), dim3(64 * kNarrowWaves), 0, st, l, b, a, parts,
+        l2_launch(kNarrow[kv_type][nq][big], dim3(plan.narrow_splits * plan.narrow_blocks, l.n_heads, b.n_seqs), dim3(64 * kNarrowWaves), 0, st, l, b, a, parts,
                   Cut{plan.narrow_splits, plan.narrow_per, plan.stride, plan.narrow_rows});
     const int most = plan.narrow_rows / group; // rows of a sequence that the narrow kernel takes
     auto join = [&](bool narrow, int blocks, int splits, int most) {

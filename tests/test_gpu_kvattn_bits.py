@@ -1,0 +1,89 @@
+"""Attention over a cache in pages: how many bits its results have, and at the ends of what the types hold, against 64-bit arithmetic."""
+import numpy as np
+import pytest
+
+from tests import kvpool_plain as plain
+from tests.kvpool_plain import BF16, F16, F32, Cache, Device, rounded
+
+pytestmark = pytest.mark.gpu
+KV = ("i8", "e4m3", "f16", "bf16")
+TINY = {F32: 2.0 ** -130, F16: 2.0 ** -25, BF16: 2.0 ** -130}
+
+
+@pytest.fixture()
+def dev():
+    from llama2_rs import _lib
+    assert _lib.lib().l2_device_count() >= 1, "no HIP device: the GPU tests cannot run"
+    d = Device()
+    yield d
+    d.close()
+
+
+def _weight(kv, t):
+    """What is left of a weight by the numbers that it enters the product as: two of 11 bits; over bf16 two of 8, three for fp32 rows."""
+    return 2.0 ** -22 if kv != "bf16" else 2.0 ** -24 if t == F32 else 2.0 ** -16
+
+
+def _bound(kv, t, q, k, v, scale, want):
+    """Element by element.  A score's products and their sum are off by a rounding each, its factors by four; the quotient by twice what the
+    score is off, by its weight's numbers, the exponential (2^-22) and the n roundings of a sum; a weight is known to no less than
+    2^-32 of the largest (times the scale of its values, which is 2^-6 of the row's largest or less)."""
+    n, D = v.shape
+    most = float((np.abs(k.astype(np.float64)) @ np.abs(q.astype(np.float64))).max() * scale)
+    score = most * ((D + 4) * 2.0 ** -24 + (2.0 ** -21 if t == F32 else 0.0))
+    s = k.astype(np.float64) @ q.astype(np.float64) * scale
+    p = np.exp(s - s.max())
+    p /= p.sum()
+    size = p @ np.abs(v.astype(np.float64))
+    off = size * (2 * score + _weight(kv, t) + 2.0 ** -21 + (n + 64) * 2.0 ** -24)
+    if kv in ("f16", "bf16"):
+        off = off + 2.0 ** -32 * p.max() * np.abs(v).sum(0)
+    else:
+        a = np.maximum(np.abs(v).max(1), 2.0 ** -60).astype(np.float64)
+        off = off + 2.0 ** -32 * (p * a).max() * (np.abs(v) / a[:, None]).sum(0)
+    return 1.01 * off + (np.abs(want) + off) * plain.HALF_STEP[t] + TINY[t]
+
+
+def _check(c, kv, t, got, q, rows, heads, scale=None, lengths=None):
+    """Every row of `got`, all of which see all positions up to their own; NaN and infinities where the formula has them."""
+    scale = c.head_size ** -0.5 if scale is None else scale
+    q, at = rounded(q, t), 0
+    for i, n in enumerate(rows):
+        k, v = c.k[c.rows_of(i)], c.v[c.rows_of(i)]
+        for j in range(n):
+            upto = c.lengths[i] - n + j + 1
+            for h in range(heads):
+                kk, vv, g = k[:upto, h // (heads // c.kv_heads)], v[:upto, h // (heads // c.kv_heads)], got[at, h]
+                want = plain.attention_row(q[at, h], kk, vv, scale)[0]
+                fine = np.isfinite(vv).all(0)
+                where = f"sequence {i} row {j} head {h}"
+                assert np.array_equal(np.isnan(g), np.isnan(want)) and np.array_equal(np.isinf(g), np.isinf(want)), where
+                np.testing.assert_array_equal(g[~np.isfinite(want)], want[~np.isfinite(want)].astype(np.float32))
+                if np.isnan(want).all():
+                    continue
+                bound = _bound(kv, t, q[at, h], kk, vv[:, fine], scale, want[fine])
+                off = np.abs(g[fine].astype(np.float64) - want[fine])
+                assert np.all(off <= bound), (where, float(np.max(off / bound)))
+            at += 1
+
+
+def _cache(dev, kv, t, lengths, k=None, v=None, seed=0, head_size=64):
+    c = Cache(dev, kv, 16, 1, head_size, lengths, seed=seed)
+    rng = np.random.default_rng(seed + 1)
+    shape = (sum(lengths), 1, head_size)
+    k = rng.standard_normal(shape).astype(np.float32) if k is None else k
+    v = rng.standard_normal(shape).astype(np.float32) if v is None else v
+    c.fill(k, v, t)
+    return c, rng
+
+
+@pytest.mark.parametrize("kv", KV)
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("lengths,rows", [([5, 12, 40, 23], [1, 3, 16, 2]), ([100], [100])])
+@pytest.mark.parametrize("head_size", [64, 128])
+def test_weights_have_more_bits_than_results(dev, kv, t, lengths, rows, head_size):
+    """Few positions with weights much alike: what a result is off by is its own rounding, and next to nothing of the weights'."""
+    c, rng = _cache(dev, kv, t, lengths, head_size=head_size)
+    q = (0.02 * rng.standard_normal((sum(rows), 2, head_size))).astype(np.float32)
+    _check(c, kv, t, c.attend(q, rows, t, 2), q, rows, 2)
+    c.close()
