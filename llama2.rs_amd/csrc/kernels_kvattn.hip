@@ -5,10 +5,11 @@
 // the fitting order; maxima and sums are a lane's own but for two exchanges, and the factors between tiles one register.  V lies transposed in the pool, so
 // nothing is transposed here.  Codes of 8 bits become 16-bit floats exactly (fp16).  Scales of keys multiply the scores, those of values the weights.
 //
-// Weights enter the second product in 16 bits, times a factor that cancels in the quotient with their sum: p_t = exp2(s_t - off).  `off` follows the tiles' max s + e, where
-// 2^e is the power of two above the largest scale of their values, so that p_t * (scale of v_t) is what is bounded, by 2^15 for fp16: off goes to 7 below max s + e, and
-// is left where it is until that lies more than 8 higher, so that sums are seldom rescaled (a tile of 32 rows would have a new maximum among them nearly always).
-// Weights are two fp16 numbers each (to within 2^-22, and no less than 2^-32 of the largest) or, over a pool in bf16, two of bf16 (2^-16) for rows of 16 bits and three for
+// Weights enter the second product in 16 bits, times a factor that cancels in the quotient with their sum: p_t = exp2(s_t - off).  `off` follows the largest s_t + log2 of the
+// scale of v_t, so that p_t * (scale of v_t) is what is bounded, by 2^15 for fp16, and the largest of these is 2^7 or more: off goes to 7 below it, and
+// is left where it is until it lies more than 8 higher, so that sums are seldom rescaled (a tile of 32 rows would have a new maximum among them nearly always).  The largest s
+// with the largest scale of a tile, which a product of less weight may have, only says whether that may be so: where it may, the positions are gone over one by one.
+// Weights, times scales, are two fp16 numbers each (to within 2^-22, and no less than 2^-32 of the largest) or, over a pool in bf16, two of bf16 (2^-16) for rows of 16 bits and three for
 // fp32 rows.  One would be what a result's own rounding is: of rows in fp16 and bf16 over pools in i8 and bf16 they then were off by 1.4 and 1.3 times what fp32 weights leave, 2.9e-4 for
 // 2.1e-4 and 2.1e-3 for 1.6e-3.  q is one number where that holds it as it is, as many as a weight for fp32 rows, two for fp16 rows over bf16; for fp16 numbers scaled by a power of two per
 // row, so that they hold what bf16 and fp32 rows may contain.
@@ -31,16 +32,18 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLeastE = -67.f; // rows whose values are held at all have scales from 2^-67
 constexpr float kBase = 7.f, kSlack = 8.f;
 
-// `off` behind a tile whose largest score times its factor is `top`, and the factor of the sums so far.
+// `off` behind a tile whose largest score times its factor, with the scale of its values, is `top`, and the factor of the sums so far.
+__device__ __forceinline__ bool raises(float off, float top) { return top - kBase > off + kSlack; }
 __device__ __forceinline__ float follow(float &off, float top) {
     const float to = top - kBase;
-    if (!(to > off + kSlack)) return 1.f; // or nothing is seen
+    if (!raises(off, top)) return 1.f; // or nothing is seen
     const float f = __builtin_amdgcn_exp2f(off - to);
     off = to;
     return f;
 }
-// 2^e above x.
+// 2^e above x; x as a power of two.
 __device__ __forceinline__ float above(float x) { return x > 0.f ? fmaxf((float)__builtin_amdgcn_frexp_expf(x), kLeastE) : kLeastE; }
+__device__ __forceinline__ float log2_of(float x) { return fmaxf(__builtin_amdgcn_logf(x), kLeastE); }
 
 // What a pool's cells become for the matrix cores: eight of them, from 8 (16) bytes.
 template <int KV>
@@ -303,6 +306,14 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
 #pragma unroll
                 for (int r = 0; r < 4; r++) mv = fmaxf(mv, vs[x][r]);
             top += above(lanes::rows_max(mv));
+            if (__ballot(raises(off, top))) {
+                top = -kInf;
+#pragma unroll
+                for (int x = 0; x < ST; x++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) top = fmaxf(top, fmaf(sc[x][r], c, log2_of(vs[x][r])));
+                top = lanes::rows_max(top);
+            }
         }
         const float f = follow(off, top);
         if (__ballot(f != 1.f)) {
@@ -521,7 +532,7 @@ __device__ __forceinline__ void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n
 // with two places for keys and three for the rest, tile i + 1 may be written from step 2 i on, and is there before 2 i + 2.
 //
 // Of heads of 128, a wave's products of a tile are 512 clocks of its matrix core per number that q is made of, and as many per number of a weight: 1536 of 16-bit rows.  Each score
-// and weight of 8-bit cells is multiplied by a scale, and conversion is the vector ALUs' too.  512 rows of 64 heads on 8 behind 7488 positions in i8: 210 us, 620 TFLOP/s of what
+// and weight of 8-bit cells is multiplied by a scale, and conversion is the vector ALUs' too.  512 rows of 64 heads on 8 behind 7488 positions in i8: 212 us, 615 TFLOP/s of what
 // one number each would take (a large library product in fp16: 1170); two prompts of 4096 and 2542, 32 heads, window 1024, bf16: 193 us, 490 TFLOP/s, of which a quarter is the last of four rounds of
 // blocks.  Weights in one number took 168 and 162.  What did not pay: one conversion spread between the products
 // (+9 %), the values' wait half a tile later, scales as float4 from LDS (16 reads a tile; they now are two registers, broadcast in rows of lanes).
@@ -756,10 +767,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
             ask_scales(sh_vs[vb], vs);
             each<32>([&](auto at) { sc[at / 16][at % 16] *= scale_at<at % 16>(ks[at / 16]); });
         }
-        float top_v = 0.f; // the largest scale of the values that the row sees
-        if (whole) {
-            if (C::kEight) top_v = fmaxf(fmaxf(sh_top[vb][0], sh_top[vb][1]), fmaxf(sh_top[vb][2], sh_top[vb][3]));
-        } else {
+        if (!whole) {
             each<32>([&](auto at) {
                 constexpr int z = at / 4, r = at % 4;
                 const int t = run_of(z) + 8 * hh;
@@ -767,15 +775,10 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
                 const bool here = bits_there >> 8 * (2 * (z / 4) + (z / 2 & 1)) & 1, see = here & seen(t0 + t + r); // run t / 16
                 const float score = sc[z / 4][4 * (z & 3) + r];
                 sc[z / 4][4 * (z & 3) + r] = see ? C::kEight ? fmaf(v_scale, 0.f, score) : score : -kInf; // NaN where the values are
-                if constexpr (C::kEight) top_v = fmaxf(top_v, see ? v_scale : 0.f);
             });
             if (C::kEight)
 #pragma unroll
                 for (int z = 0; z < 2; z++) vs[z] = vs[z] == vs[z] ? vs[z] : 0.f; // nothing of a row that is not seen
-            if (C::kEight) {
-                const lanes::Both v2 = lanes::both32(top_v);
-                top_v = fmaxf(v2.lo, v2.hi);
-            }
         }
         float mx = -kInf;
 #pragma unroll
@@ -784,7 +787,16 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
             for (int r = 0; r < 4; r++) mx = fmaxf(mx, sc[z / 4][4 * (z & 3) + r]);
         const lanes::Both m2 = lanes::both32(mx);
         float top = fmaxf(m2.lo, m2.hi) * c;
-        if (C::kEight) top += above(top_v);
+        if constexpr (C::kEight) {
+            if (whole) top += above(fmaxf(fmaxf(sh_top[vb][0], sh_top[vb][1]), fmaxf(sh_top[vb][2], sh_top[vb][3])));
+            if (!whole || __ballot(raises(off, top))) {
+                const float e[2] = {log2_of(vs[0]), log2_of(vs[1])};
+                mx = -kInf;
+                each<32>([&](auto at) { mx = fmaxf(mx, fmaf(sc[at / 16][at % 16], c, scale_at<at % 16>(e[at / 16]))); });
+                const lanes::Both e2 = lanes::both32(mx);
+                top = fmaxf(e2.lo, e2.hi);
+            }
+        }
         const float f = follow(off, top);
         if (__ballot(f != 1.f)) {
 #pragma unroll

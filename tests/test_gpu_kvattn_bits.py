@@ -87,3 +87,28 @@ def test_weights_have_more_bits_than_results(dev, kv, t, lengths, rows, head_siz
     q = (0.02 * rng.standard_normal((sum(rows), 2, head_size))).astype(np.float32)
     _check(c, kv, t, c.attend(q, rows, t, 2), q, rows, 2)
     c.close()
+
+
+@pytest.mark.parametrize("kv", ["i8", "e4m3"])
+@pytest.mark.parametrize("t", [F32, F16])
+@pytest.mark.parametrize("lengths,rows", [([2, 90, 200], [1, 2, 3]), ([150], [100])])
+@pytest.mark.parametrize("ratio", [0, 10, 17, 24, 45])
+def test_large_values_of_next_to_no_weight(dev, kv, t, lengths, rows, ratio):
+    """Values 2^ratio times the others', of rows whose weight is e^-50 of the others': those keep their bits."""
+    rng = np.random.default_rng(ratio)
+    n, D = sum(lengths), 64
+    ratio = min(ratio, 13) if t == F16 else ratio
+    k, v = np.zeros((n, 1, D), np.float32), rng.standard_normal((n, 1, D)).astype(np.float32)
+    large = np.zeros(n, bool)
+    at = 0
+    for m in lengths:
+        large[[at + x for x in (0, 40, 41, 64, 100) if x < m]] = True
+        at += m
+    k[:, 0, 1] = 0.01 * rng.standard_normal(n)
+    k[large, 0, 0] = -50
+    v[large] *= np.float32(2.0 ** ratio)
+    c, _ = _cache(dev, kv, t, lengths, k, v)
+    q = np.zeros((sum(rows), 2, D), np.float32)
+    q[..., 0], q[..., 1] = 8, rng.standard_normal((sum(rows), 2))
+    _check(c, kv, t, c.attend(q, rows, t, 2), q, rows, 2)
+    c.close()
