@@ -45,6 +45,19 @@ __device__ __forceinline__ float follow(float &off, float top) {
 __device__ __forceinline__ float above(float x) { return x > 0.f ? fmaxf((float)__builtin_amdgcn_frexp_expf(x), kLeastE) : kLeastE; }
 __device__ __forceinline__ float log2_of(float x) { return fmaxf(__builtin_amdgcn_logf(x), kLeastE); }
 
+// Of a row of q whose largest number is `top`: times 2^e for fp16, and `c`, the exponent of two per unit of the scores' sums, times scales (of keys) that come as scale_of_key().
+// The largest number of q is in [2^14, 2^15), or as far below as it takes for c to be a normal number: a c of zero would make NaN of a score that is not seen, and
+// scores that so small a factor goes with are next to zero.  Sums times scales are up to 2^152 of i8, hence the 2^-24.
+template <bool EIGHT>
+__device__ __forceinline__ int fit_q(float top, float &c) {
+    constexpr int kKey = EIGHT ? 24 : 0;
+    const int most = 125 + kKey + __builtin_amdgcn_frexp_expf(c);
+    const int e = min(top > 0.f && top < kInf ? 15 - __builtin_amdgcn_frexp_expf(top) : 0, most);
+    c = fminf(ldexpf(c, kKey - e), 0x1p127f); // at 2^127 scores are far apart or the same
+    return e;
+}
+__device__ __forceinline__ float scale_of_key(float s) { return s * 0x1p-24f; }
+
 // What a pool's cells become for the matrix cores: eight of them, from 8 (16) bytes.
 template <int KV>
 struct Cells {
@@ -246,12 +259,11 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
         c = a.scale * kLog2e;
         if (C::kHalf) {
             top = lanes::rows_max(top);
-            const int e = top > 0.f && top < kInf ? 15 - __builtin_amdgcn_frexp_expf(top) : 0; // the largest in [2^14, 2^15)
+            const int e = fit_q<C::kEight>(top, c);
 #pragma unroll
             for (int k = 0; k < D / 32; k++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) x[k][j] = ldexpf(x[k][j], e);
-            c = ldexpf(c, -e);
         }
 #pragma unroll
         for (int k = 0; k < D / 32; k++) pieces<Frag, typename C::One, NQ>(x[k], q[k]);
@@ -273,7 +285,9 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
             }
         if (C::kEight)
 #pragma unroll
-            for (int x = 0; x < ST; x++) sc[x] *= ks[x];
+            for (int x = 0; x < ST; x++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) sc[x][r] *= scale_of_key(ks[x][r]);
         const int here_next = page_v;
         if (more) load_k(n + kNarrowWaves, page_k, page_v);
 
@@ -532,7 +546,7 @@ __device__ __forceinline__ void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n
 // with two places for keys and three for the rest, tile i + 1 may be written from step 2 i on, and is there before 2 i + 2.
 //
 // Of heads of 128, a wave's products of a tile are 512 clocks of its matrix core per number that q is made of, and as many per number of a weight: 1536 of 16-bit rows.  Each score
-// and weight of 8-bit cells is multiplied by a scale, and conversion is the vector ALUs' too.  512 rows of 64 heads on 8 behind 7488 positions in i8: 212 us, 615 TFLOP/s of what
+// and weight of 8-bit cells is multiplied by a scale, and conversion is the vector ALUs' too.  512 rows of 64 heads on 8 behind 7488 positions in i8: 207 us, 630 TFLOP/s of what
 // one number each would take (a large library product in fp16: 1170); two prompts of 4096 and 2542, 32 heads, window 1024, bf16: 193 us, 490 TFLOP/s, of which a quarter is the last of four rounds of
 // blocks.  Weights in one number took 168 and 162.  What did not pay: one conversion spread between the products
 // (+9 %), the values' wait half a tile later, scales as float4 from LDS (16 reads a tile; they now are two registers, broadcast in rows of lanes).
@@ -605,8 +619,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
             }
             const lanes::Both t = lanes::both32(top);
             top = fmaxf(t.lo, t.hi);
-            e = top > 0.f && top < kInf ? 15 - __builtin_amdgcn_frexp_expf(top) : 0; // the largest in [2^14, 2^15)
-            c = ldexpf(c, -e);
+            e = fit_q<C::kEight>(top, c);
         }
 #pragma unroll
         for (int k = 0; k < KS; k++) {
@@ -765,6 +778,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
         const bool odd = !C::kEight && sh_odd[vb] == x;
         if constexpr (C::kEight) {
             ask_scales(sh_vs[vb], vs);
+            ks[0] = scale_of_key(ks[0]), ks[1] = scale_of_key(ks[1]);
             each<32>([&](auto at) { sc[at / 16][at % 16] *= scale_at<at % 16>(ks[at / 16]); });
         }
         if (!whole) {

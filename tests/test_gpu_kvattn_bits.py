@@ -112,3 +112,30 @@ def test_large_values_of_next_to_no_weight(dev, kv, t, lengths, rows, ratio):
     q[..., 0], q[..., 1] = 8, rng.standard_normal((sum(rows), 2))
     _check(c, kv, t, c.attend(q, rows, t, 2), q, rows, 2)
     c.close()
+
+
+@pytest.mark.parametrize("kv", KV)
+@pytest.mark.parametrize("t,size,scale", [(F32, 1e-41, None), (F32, 2.0 ** -149, None), (F32, 1e-12, 1e-30), (F32, 1e-38, 1e-38), (BF16, 2.0 ** -133, 1e-6),
+                                          (BF16, 1e-38, None), (F16, 2.0 ** -24, 1e-36), (F32, 2.0 ** 100, 2.0 ** -100), (F32, 1e-20, 1e-44)])
+@pytest.mark.parametrize("lengths,rows", [([5, 90, 37], [1, 3, 2]), ([130], [100])])
+def test_factors_at_the_ends_of_fp32(dev, kv, t, size, scale, lengths, rows):
+    """Queries and scales whose product is next to nothing, or which lie far apart: what is not seen stays out, and scores are what they are."""
+    c, rng = _cache(dev, kv, t, lengths)
+    q = (size * np.sign(rng.standard_normal((sum(rows), 2, 64)))).astype(np.float32)
+    scale = None if scale is None else float(np.float32(scale))
+    got = c.attend(q, rows, t, 2, scale=scale or 0.0)
+    assert np.isfinite(got).all()
+    _check(c, kv, t, got, q, rows, 2, scale)
+    c.close()
+
+
+@pytest.mark.parametrize("kv", ["i8", "e4m3", "bf16"])
+@pytest.mark.parametrize("lengths,rows", [([5, 90, 37], [1, 3, 2]), ([130], [100])])
+def test_keys_of_1e33(dev, kv, lengths, rows):
+    """Large keys and small queries: scores are small, whatever the sums before the factors are."""
+    rng = np.random.default_rng(3)
+    k = (2.0 ** 110 * rng.standard_normal((sum(lengths), 1, 64))).astype(np.float32)
+    c, _ = _cache(dev, kv, F32, lengths, k)
+    q = (2.0 ** -111 * rng.standard_normal((sum(rows), 2, 64))).astype(np.float32)
+    _check(c, kv, F32, c.attend(q, rows, F32, 2), q, rows, 2)
+    c.close()
