@@ -278,7 +278,8 @@ int l2_kvpool_read(l2_kvpool *p, int layer, const l2_kvbatch *batch, void *k_dev
  * zeros where nothing is seen.  Keys and values come from the pool, those of the rows included (l2_kvpool_write first).  Scores, statistics and sums
  * are fp32; q of 16 bits enters the matrix cores as it is, fp32 q and all weights of the softmax as several 16-bit numbers: to within 2^-22
  * (over L2_KV_BF16 2^-24, for 16-bit rows 2^-16), a weight also, but over L2_KV_BF16, to no less than 2^-32 of the largest, in 8 bits each times the scale of its values.  What is not seen has no influence, NaN and infinities included.
- * Scores are good up to 2^22 in magnitude. */
+ * A value that is not finite makes its dimension the sum of those; a row that sees a key with infinities may be NaN where the formula is not.  Scores are good
+ * up to 2^22 in magnitude. */
 typedef struct l2_attention {
     int32_t n_heads;
     int32_t type;       /* L2_F32, L2_F16 or L2_BF16 */

@@ -13,6 +13,8 @@
 // fp32 rows.  One would be what a result's own rounding is: of rows in fp16 and bf16 over pools in i8 and bf16 they then were off by 1.4 and 1.3 times what fp32 weights leave, 2.9e-4 for
 // 2.1e-4 and 2.1e-3 for 1.6e-3.  q is one number where that holds it as it is, as many as a weight for fp32 rows, two for fp16 rows over bf16; for fp16 numbers scaled by a power of two per
 // row, so that they hold what bf16 and fp32 rows may contain.
+// Values of 16 bits that are not finite would be NaN times the second number of a weight, or times one that is zero, and for rows that do not see them: they are taken out of
+// tiles that some row may not see whole, and sums that are not finite behind the last tile, or lack some, are made from the values that are not (repair).
 #include <algorithm>
 
 #include "kvpool.h"
@@ -151,6 +153,20 @@ __device__ __forceinline__ u4 finite(u4 v, bool &odd) {
     return v;
 }
 
+// The sums of a row over tiles whose values may not be finite: those that are not finite as a number that no sum is, so that a value that the row sees makes it that, or NaN;
+// and what is left behind all values.
+constexpr float kBroken = 0x1.fffffep127f;
+__device__ __forceinline__ float broken(float sum) { return fabsf(sum) < kInf ? sum : kBroken; }
+__device__ __forceinline__ float mended(float sum) { return sum == kBroken ? __builtin_nanf("") : sum; }
+// A cell that is not finite, or else zero.
+template <int KV>
+__device__ __forceinline__ float not_finite(uint16_t bits) {
+    const float v = KV == L2_KV_F16 ? (float)__builtin_bit_cast(_Float16, bits) : kv::bf16_float(bits);
+    return fabsf(v) < kInf ? 0.f : v;
+}
+// A part's sum times its factor, which may be zero.
+__device__ __forceinline__ float times(float sum, float f) { return fabsf(sum) < kInf ? sum * f : sum; }
+
 constexpr int kNarrowRows = 16, kNarrowWaves = 4;
 
 // The numbers that a weight is, of rows whose q is NQ.
@@ -271,6 +287,7 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
 
     f4 acc[DT] = {};
     float off = -kInf, sum = 0.f;
+    bool odd = false; // values were taken out
     for (; n < end; n += kNarrowWaves) {
         const int t0 = range.tile(n) * TT;
         const bool more = n + kNarrowWaves < end;
@@ -293,7 +310,6 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
 
         // positions CH g + 4 x + r of the tile are this lane's
         const bool whole = t0 + TT - 1 <= base && (!a.window || t0 > s.length - 1 - a.window || t0 + TT <= a.sinks) && __ballot(here < 0) == 0;
-        bool odd = false; // a value that is not finite where some row may not see it
         if (!whole) {
 #pragma unroll
             for (int x = 0; x < ST; x++)
@@ -354,24 +370,6 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
                 for (int y = 0; y < NP; y++) acc[x] = mfma16(fr, pf[y], acc[x]);
             }
         }
-        if (__ballot(odd)) { // added one by one, to the rows that see them
-#pragma unroll 1
-            for (int y = 0; y < TT; y++) {
-                const int t = t0 + y, page = kv::page_at(b, l.n_pages, i, t >> l.page_shift);
-                if (page < 0 || !seen(t)) continue;
-                int first = 4 * g; // unknown, so that the places are not worked out ahead of the loop
-                asm volatile("" : "+v"(first));
-                const uint16_t *p = (const uint16_t *)vb + (((int64_t)page * l.n_heads + h) * D * size + (t & (size - 1)));
-#pragma unroll
-                for (int x = 0; x < DT; x++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const uint16_t bits = p[(int64_t)(16 * x + first + r) * size];
-                        const float v = KV == L2_KV_F16 ? (float)__builtin_bit_cast(_Float16, bits) : kv::bf16_float(bits);
-                        if (!(fabsf(v) < kInf)) acc[x][r] += v;
-                    }
-            }
-        }
         here = here_next;
         if (more) {
             load_v(n + kNarrowWaves, page_v);
@@ -379,6 +377,32 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
         }
     }
     sum = lanes::rows_sum(sum);
+    if constexpr (!C::kEight) {
+#pragma unroll
+        for (int x = 0; x < DT; x++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) odd |= !(fabsf(acc[x][r]) < kInf);
+        if (__ballot(odd)) { // repair: position by position
+#pragma unroll
+            for (int x = 0; x < DT; x++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[x][r] = broken(acc[x][r]);
+#pragma unroll 1
+            for (int y = TT * (begin + w); y < TT * end; y += y % TT == TT - 1 ? TT * (kNarrowWaves - 1) + 1 : 1) {
+                const int t = range.tile(y / TT) * TT + y % TT, page = kv::page_at(b, l.n_pages, i, t >> l.page_shift);
+                if (page < 0 || !seen(t)) continue;
+                const uint16_t *p = (const uint16_t *)vb + ((((int64_t)page * l.n_heads + h) * D + 4 * g) * size + (t & (size - 1)));
+#pragma unroll
+                for (int x = 0; x < DT; x++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc[x][r] += not_finite<KV>(p[(int64_t)(16 * x + r) * size]);
+            }
+#pragma unroll
+            for (int x = 0; x < DT; x++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[x][r] = mended(acc[x][r]);
+        }
+    }
 
     // the waves' parts together
     constexpr int LD = D + 4;
@@ -400,7 +424,8 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
             const float f = st.x == o ? 1.f : __builtin_amdgcn_exp2f(st.x - o);
             if (st.y == 0.f && st.x == -kInf) continue;
             total += st.y * f;
-            v += *(const f4 *)&sh_acc[y][r][d] * f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] += times(sh_acc[y][r][d + j], f);
         }
         const int64_t row = s.first + (r0 + r) / group, hq = h * group + (r0 + r) % group;
         if (cut.splits == 1) {
@@ -471,7 +496,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void kv_join_kernel(l2_kvbatch b, 
             sum += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), x));
             if (__builtin_amdgcn_readlane(is, x))
 #pragma unroll
-                for (int e = 0; e < E; e++) v[e] += part[x][e] * fx;
+                for (int e = 0; e < E; e++) v[e] += times(part[x][e], fx);
         }
 #pragma unroll
         for (int e = 0; e < E; e++) kv::store(a.out, a.type, row * a.out_stride + (int64_t)hq * D + E * lane + e, sum == 0.f ? 0.f : v[e] / sum);
@@ -490,7 +515,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void kv_join_kernel(l2_kvbatch b, 
             const float f = none(st) ? 0.f : st.x == o ? 1.f : __builtin_amdgcn_exp2f(st.x - o);
             total += none(st) ? 0.f : st.y * f;
 #pragma unroll
-            for (int e = 0; e < E; e++) v[e] += none(st) ? 0.f : part[e] * f;
+            for (int e = 0; e < E; e++) v[e] += none(st) ? 0.f : times(part[e], f);
         }
 #pragma unroll
         for (int e = 0; e < E; e++) sh_acc[w][E * lane + e] = v[e];
@@ -559,7 +584,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
     __shared__ __align__(16) float sh_ks[3][TT], sh_vs[3][TT];
     __shared__ __align__(16) float sh_top[3][4];
     __shared__ uint32_t sh_there[3];
-    __shared__ int sh_seq, sh_tile, sh_odd[3];
+    __shared__ int sh_seq, sh_tile, sh_odd;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, hh = lane >> 5;
     const int group = a.n_heads / l.n_heads;
     const int h = __builtin_amdgcn_readfirstlane(blockIdx.x % l.n_heads), split = __builtin_amdgcn_readfirstlane(blockIdx.x / l.n_heads % cut.splits);
@@ -567,8 +592,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
     // which sequence's rows: the tiles of all sequences one behind the other
     {
         int at = blockIdx.x / (l.n_heads * cut.splits);
-        if (tid == 0) sh_seq = -1;
-        if (tid < 3) sh_odd[tid] = -1;
+        if (tid == 0) sh_seq = -1, sh_odd = 0;
         __syncthreads();
         for (int i0 = 0; i0 < b.n_seqs; i0 += 64) {
             int tiles = 0;
@@ -685,7 +709,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
         if (x + 1 < end) ask_page(x + 1);
     };
     // Has this wave's run of tile x + by, asked for before, in LDS.  16-bit cells get there by themselves: where a row may not see all of the tile, values that
-    // are not finite are taken out (and added to the rows that do see them, one by one).
+    // are not finite are taken out.
     auto put = [&](int x, int by) {
         x += by;
         if (x >= end) return;
@@ -713,7 +737,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
                 bool odd = false;
                 u4 *at = &sh_v[vb][2 * D * run + 64 * y + lane];
                 const u4 v = finite<KV>(*at, odd);
-                if (odd) *at = v, sh_odd[vb] = x;
+                if (odd) *at = v, sh_odd = 1;
             }
         }
     };
@@ -775,7 +799,6 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
         const int vb = cur, t0 = range.tile(x) * TT;
         const uint32_t bits_there = __builtin_amdgcn_readfirstlane(runs);
         const bool whole = bits_there == 0x01010101 && all_visible(t0, w_first, w_last);
-        const bool odd = !C::kEight && sh_odd[vb] == x;
         if constexpr (C::kEight) {
             ask_scales(sh_vs[vb], vs);
             ks[0] = scale_of_key(ks[0]), ks[1] = scale_of_key(ks[1]);
@@ -833,26 +856,6 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
         for (int v = 0; v < 4; v++)
 #pragma unroll
             for (int y = 0; y < NP; y++) asm volatile("" : "+v"(pf[v][y]));
-        if (odd) {
-#pragma unroll 1
-            for (int y = 0; y < TT; y++) {
-                const int t = t0 + y, page = kv::page_at(b, l.n_pages, i, t >> l.page_shift);
-                if (page < 0 || !seen(t)) continue;
-                int half = hh; // unknown, so that 64 places are not worked out ahead of the loop
-                asm volatile("" : "+v"(half));
-                const uint16_t *cells = (const uint16_t *)l.v + (((int64_t)page * l.n_heads + h) * D * size + (t & (size - 1)));
-#pragma unroll
-                for (int z = 0; z < DT; z++) {
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const uint16_t bits = cells[(int64_t)(32 * z + 8 * (r / 4) + 4 * half + r % 4) * size];
-                        const float v = KV == L2_KV_F16 ? (float)__builtin_bit_cast(_Float16, bits) : kv::bf16_float(bits);
-                        if (!(fabsf(v) < kInf)) acc[z][r] += v;
-                    }
-                    asm volatile("" ::: "memory");
-                }
-            }
-        }
     };
 
     if (begin < end) {
@@ -896,6 +899,33 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
         barrier();
         products(yes, no, cur, 0);
         if (!late) barrier();
+    }
+    if constexpr (!C::kEight) { // as in the narrow kernel
+        bool odd = begin < end && sh_odd;
+#pragma unroll
+        for (int y = 0; y < DT; y++)
+#pragma unroll
+            for (int z = 0; z < 16; z++) odd |= !(fabsf(acc[y][z]) < kInf);
+        if (__ballot(odd)) {
+#pragma unroll
+            for (int y = 0; y < DT; y++)
+#pragma unroll
+                for (int z = 0; z < 16; z++) acc[y][z] = broken(acc[y][z]);
+#pragma unroll 1
+            for (int x = TT * begin; x < TT * end; x++) {
+                const int t = range.tile(x / TT) * TT + x % TT, page = kv::page_at(b, l.n_pages, i, t >> l.page_shift);
+                if (page < 0 || !seen(t)) continue;
+                const uint16_t *p = (const uint16_t *)l.v + ((((int64_t)page * l.n_heads + h) * D + 4 * hh) * size + (t & (size - 1)));
+#pragma unroll
+                for (int y = 0; y < DT; y++)
+#pragma unroll
+                    for (int z = 0; z < 16; z++) acc[y][z] += not_finite<KV>(p[(int64_t)(32 * y + 8 * (z / 4) + z % 4) * size]);
+            }
+#pragma unroll
+            for (int y = 0; y < DT; y++)
+#pragma unroll
+                for (int z = 0; z < 16; z++) acc[y][z] = mended(acc[y][z]);
+        }
     }
     const lanes::Both s2 = lanes::both32(sum);
     sum = s2.lo + s2.hi;

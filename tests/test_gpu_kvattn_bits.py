@@ -139,3 +139,23 @@ def test_keys_of_1e33(dev, kv, lengths, rows):
     q = (2.0 ** -111 * rng.standard_normal((sum(rows), 2, 64))).astype(np.float32)
     _check(c, kv, F32, c.attend(q, rows, F32, 2), q, rows, 2)
     c.close()
+
+
+@pytest.mark.parametrize("kv", ["f16", "bf16"])
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("lengths,rows", [([1500], [1]), ([70, 400], [3, 2]), ([300], [100])])
+def test_infinite_values_that_are_seen(dev, kv, t, lengths, rows):
+    """An infinity in a dimension of values makes the result that, and NaN NaN, whatever its weight and how many rows see its tile; both infinities are NaN; other dimensions
+    are as they were."""
+    rng = np.random.default_rng(5)
+    n = sum(lengths)
+    k, v = (rng.standard_normal((n, 1, 64)).astype(np.float32) for _ in "kv")
+    inf = np.inf
+    v[2, 0, 5], v[3, 0, 6], v[9, 0, 6], v[20, 0, 7], v[21, 0, 8], v[40, 0, 9], v[40, 0, 63] = inf, -inf, inf, -inf, np.nan, inf, -inf
+    v[n - 20, 0, 10], v[n - 1, 0, 11] = -inf, inf
+    k[20, 0], k[40, 0] = -20, 20
+    c, _ = _cache(dev, kv, t, lengths, k, v)
+    q = rng.standard_normal((sum(rows), 2, 64)).astype(np.float32)
+    q[:, 0] = 1  # the keys of 20 and 40 decide nearly alone
+    _check(c, kv, t, c.attend(q, rows, t, 2), q, rows, 2)
+    c.close()
