@@ -6,7 +6,7 @@
 // nothing is transposed here.  Codes of 8 bits become 16-bit floats exactly (fp16).  Scales of keys multiply the scores, those of values the weights.
 //
 // Weights enter the second product in 16 bits, times a factor that cancels in the quotient with their sum: p_t = exp2(s_t - off).  `off` follows the largest s_t + log2 of the
-// scale of v_t, so that p_t * (scale of v_t) is what is bounded, by 2^15 for fp16, and the largest of these is 2^7 or more: off goes to 7 below it, and
+// scale of v_t, so that p_t * (scale of v_t) is what is bounded, by 2^15 for fp16, and the largest of these is 2^7 or more (over bf16, of values up to 2^127, 1 and 2^-8): off goes to 7 below it, and
 // is left where it is until it lies more than 8 higher, so that sums are seldom rescaled (a tile of 32 rows would have a new maximum among them nearly always).  The largest s
 // with the largest scale of a tile, which a product of less weight may have, only says whether that may be so: where it may, the positions are gone over one by one.
 // Weights, times scales, are two fp16 numbers each (to within 2^-22, and no less than 2^-32 of the largest) or, over a pool in bf16, two of bf16 (2^-16) for rows of 16 bits and three for
@@ -32,13 +32,18 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLeastE = -67.f; // rows whose values are held at all have scales from 2^-67
-constexpr float kBase = 7.f, kSlack = 8.f;
+constexpr float kSlack = 8.f;
+constexpr float base_of(int kv_type) { return kv_type == L2_KV_BF16 ? -8.f : 7.f; }
 
 // `off` behind a tile whose largest score times its factor, with the scale of its values, is `top`, and the factor of the sums so far.
-__device__ __forceinline__ bool raises(float off, float top) { return top - kBase > off + kSlack; }
+template <int KV>
+__device__ __forceinline__ bool raises(float off, float top) {
+    return top - base_of(KV) > off + kSlack;
+}
+template <int KV>
 __device__ __forceinline__ float follow(float &off, float top) {
-    const float to = top - kBase;
-    if (!raises(off, top)) return 1.f; // or nothing is seen
+    const float to = top - base_of(KV);
+    if (!raises<KV>(off, top)) return 1.f; // or nothing is seen
     const float f = __builtin_amdgcn_exp2f(off - to);
     off = to;
     return f;
@@ -336,7 +341,7 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
 #pragma unroll
                 for (int r = 0; r < 4; r++) mv = fmaxf(mv, vs[x][r]);
             top += above(lanes::rows_max(mv));
-            if (__ballot(raises(off, top))) {
+            if (__ballot(raises<KV>(off, top))) {
                 top = -kInf;
 #pragma unroll
                 for (int x = 0; x < ST; x++)
@@ -345,7 +350,7 @@ __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer
                 top = lanes::rows_max(top);
             }
         }
-        const float f = follow(off, top);
+        const float f = follow<KV>(off, top);
         if (__ballot(f != 1.f)) {
 #pragma unroll
             for (int x = 0; x < DT; x++) acc[x] *= f;
@@ -826,7 +831,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
         float top = fmaxf(m2.lo, m2.hi) * c;
         if constexpr (C::kEight) {
             if (whole) top += above(fmaxf(fmaxf(sh_top[vb][0], sh_top[vb][1]), fmaxf(sh_top[vb][2], sh_top[vb][3])));
-            if (!whole || __ballot(raises(off, top))) {
+            if (!whole || __ballot(raises<KV>(off, top))) {
                 const float e[2] = {log2_of(vs[0]), log2_of(vs[1])};
                 mx = -kInf;
                 each<32>([&](auto at) { mx = fmaxf(mx, fmaf(sc[at / 16][at % 16], c, scale_at<at % 16>(e[at / 16]))); });
@@ -834,7 +839,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_
                 top = fmaxf(e2.lo, e2.hi);
             }
         }
-        const float f = follow(off, top);
+        const float f = follow<KV>(off, top);
         if (__ballot(f != 1.f)) {
 #pragma unroll
             for (int y = 0; y < DT; y++) acc[y] *= f;

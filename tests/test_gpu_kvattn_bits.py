@@ -159,3 +159,15 @@ def test_infinite_values_that_are_seen(dev, kv, t, lengths, rows):
     q[:, 0] = 1  # the keys of 20 and 40 decide nearly alone
     _check(c, kv, t, c.attend(q, rows, t, 2), q, rows, 2)
     c.close()
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("lengths,rows", [([5, 90, 37], [1, 3, 2]), ([130], [100])])
+def test_values_of_1e36_in_bf16(dev, t, lengths, rows):
+    """The sum of weights times values stays finite where their mean is."""
+    rng = np.random.default_rng(6)
+    v = (2.0 ** 117 * rng.standard_normal((sum(lengths), 1, 64))).astype(np.float32)
+    c, _ = _cache(dev, "bf16", t, lengths, None, v)
+    q = rng.standard_normal((sum(rows), 2, 64)).astype(np.float32)
+    _check(c, "bf16", t, c.attend(q, rows, t, 2), q, rows, 2)
+    c.close()
