@@ -171,3 +171,37 @@ def test_values_of_1e36_in_bf16(dev, t, lengths, rows):
     q = rng.standard_normal((sum(rows), 2, 64)).astype(np.float32)
     _check(c, "bf16", t, c.attend(q, rows, t, 2), q, rows, 2)
     c.close()
+
+
+@pytest.mark.parametrize("kv", KV)
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("lengths,rows", [([700], [1]), ([70, 150], [20, 3]), ([150], [100])])
+def test_keys_and_queries_that_are_not_finite(dev, kv, t, lengths, rows):
+    """NaN in a key or a query makes every row NaN that sees it, or is it, and no other; an infinity no number where the formula has none."""
+    rng = np.random.default_rng(7)
+    n = sum(lengths)
+    k = rng.standard_normal((n, 1, 64)).astype(np.float32)
+    k[n - 2, 0, 3] = np.nan
+    if len(lengths) > 1:
+        k[lengths[0] - 5, 0, 4] = np.inf
+    c, _ = _cache(dev, kv, t, lengths, k)
+    q = rng.standard_normal((sum(rows), 2, 64)).astype(np.float32)
+    q[0, 1, 9] = np.nan
+    got = c.attend(q, rows, t, 2)
+    at = 0
+    for i, m in enumerate(rows):
+        for j in range(m):
+            upto = lengths[i] - m + j + 1
+            kk, vv = c.k[c.rows_of(i)][:upto, 0], c.v[c.rows_of(i)][:upto, 0]
+            for h in range(2):
+                qq = rounded(q[at, h], t)
+                if np.isnan(kk).any() or np.isnan(qq).any():
+                    assert np.isnan(got[at, h]).all(), (i, j, h)
+                elif not np.isfinite(kk).all():
+                    want = plain.attention_row(qq, kk, vv, 0.125)[0]
+                    assert np.isnan(got[at, h]).all() or np.isfinite(want).all(), (i, j, h)
+                else:
+                    want = plain.attention_row(qq, kk, vv, 0.125)[0]
+                    assert np.all(np.abs(got[at, h] - want) <= _bound(kv, t, qq, kk, vv, 0.125, want)), (i, j, h)
+            at += 1
+    c.close()
