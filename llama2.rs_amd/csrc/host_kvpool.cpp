@@ -69,7 +69,8 @@ extern "C" int l2_kvpool_create(int n_layers, int n_pages, int page_size, int n_
     if (kv_type < L2_KV_I8 || kv_type > L2_KV_BF16) return l2_fail(L2_ERR_ARG, "kv type %d", kv_type);
     const bool eight = kv_type <= L2_KV_E4M3;
     const size_t rows = (size_t)n_pages * page_size * n_kv_heads; // below 2^31 * 2^8 * 2^16
-    if (rows >= (size_t)1 << 44 || (size_t)n_layers * rows >= (size_t)1 << 44) return l2_fail(L2_ERR_RANGE, "a pool of more than 2^44 rows");
+    constexpr size_t kMost = ((size_t)1 << 44) - 1;
+    if (rows > kMost || (size_t)n_layers > kMost / rows) return l2_fail(L2_ERR_RANGE, "a pool of more than 2^44 rows");
     int n = 0;
     const hipError_t e = hipGetDeviceCount(&n);
     if (e != hipSuccess || n < 1) {
