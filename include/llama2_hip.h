@@ -306,7 +306,7 @@ int l2_kvpool_attention(l2_kvpool *p, int layer, const l2_kvbatch *batch, const 
  * The first is always kept.  The answer is the first id, in the vocabulary's order, at which the running sum of the kept weights passes u times
  * their sum (Random::sample, src/util.rs:102-113); of a u of 1 or more the last kept, and a u below 0 or NaN is 0.  A temperature of 0 (or below, or NaN) takes the first token.  Weights are whole multiples of 2^-44 and sums of them
  * exact, so a row's answer is the same in every batch and call.  NaN logits count as -infinity; a row with nothing else gets -1.  An infinite
- * logit shares everything with its equals.  vocab up to 2^19.  ids_dev is host-visible or device memory.
+ * logit shares everything with its equals.  vocab up to 2^19, rows up to 2^21.  ids_dev is host-visible or device memory.
  * Enqueued on hip_stream without waiting; allocates nothing; may be captured (after a first call, or l2_kvpool_create, on the device).
  * temperature, top_k, top_p, min_p and u are device arrays [rows]; any of the first four may be NULL: 1, off, off, off. */
 typedef struct l2_sampling {

@@ -209,6 +209,7 @@ extern "C" int l2_sample_device(const void *logits_dev, int type, int rows, int 
     if (!s) return l2_fail(L2_ERR_ARG, "null argument");
     L2_TRY(check_type(type));
     if (rows < 0 || vocab < 1 || vocab > kMaxVocab) return l2_fail(L2_ERR_ARG, "%d rows of %d logits (up to 2^19)", rows, vocab);
+    if (rows > 1 << 21) return l2_fail(L2_ERR_RANGE, "%d rows (up to 2^21)", rows); // blocks of 2^10 threads, of which a launch has fewer than 2^32
     L2_TRY(check_stride(&stride, vocab, "stride"));
     if (rows == 0) return L2_OK;
     if (!logits_dev || !ids_dev || !s->u) return l2_fail(L2_ERR_ARG, "null argument");

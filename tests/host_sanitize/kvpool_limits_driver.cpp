@@ -19,8 +19,18 @@ static void pools_past_64_bits() {
     no_memory = false;
 }
 
+// Rows of logits, a block of 1024 threads each: a launch takes fewer than 2^32.
+static void rows_past_32_bits() {
+    float x[1] = {};
+    int32_t ids[1];
+    const l2_sampling s{nullptr, nullptr, nullptr, nullptr, x};
+    for (int rows : {(1 << 21) + 1, 1 << 22, 0x7FFFFFFF}) REFUSED(L2_ERR_RANGE, l2_sample_device((void *)64, L2_F32, rows, 1, 0, &s, ids, nullptr));
+    REQUIRE(l2_sample_device((void *)64, L2_F32, 1 << 21, 1, 0, &s, ids, nullptr) == L2_OK);
+}
+
 int main() {
     pools_past_64_bits();
+    rows_past_32_bits();
     puts("ok");
     return 0;
 }
