@@ -289,6 +289,7 @@ typedef struct l2_attention {
     int64_t q_stride;   /* elements from row to row; 0: dense */
     int64_t out_stride;
 } l2_attention;
+/* L2_ERR_RANGE where chunks may make 2^23 blocks or more, of 256 rows and query heads of a kv head (a sequence's last fewer). */
 /* Bytes of device memory that such a call wants as its workspace (aligned to 16; its contents do not matter before the call and mean nothing
  * behind it).  They follow from the limits in `batch`, not from its arrays.  May be 0. */
 int l2_kvpool_attention_workspace(const l2_kvpool *p, const l2_kvbatch *batch, const l2_attention *a, size_t *bytes);

@@ -1022,7 +1022,7 @@ int kv_attention_launch(const KvLayer &l, int kv_type, const l2_kvbatch &b, cons
     parts.stat = (float2 *)(parts.acc + (size_t)b.n_rows * a.n_heads * plan.stride * l.head_size);
     if (plan.wide && plan.wide_tiles) {
         const int64_t blocks = plan.wide_tiles * l.n_heads * plan.wide_splits;
-        if (blocks >= (int64_t)1 << 31) return l2_fail(L2_ERR_RANGE, "%d rows of %d heads", b.n_rows, a.n_heads);
+        if (blocks >= ((int64_t)1 << 32) / kWideThreads) return l2_fail(L2_ERR_RANGE, "%d rows of %d heads", b.n_rows, a.n_heads); // a launch has fewer than 2^32 threads
         l2_launch(kWide[kv_type][nq][big], dim3((unsigned)blocks), dim3(kWideThreads), 0, st, l, b, a, parts,
                   Cut{plan.wide_splits, plan.wide_per, plan.stride, plan.narrow_rows});
     }

@@ -26,3 +26,7 @@ def _run(tmp_path, driver, flags):
 
 def test_calls_past_the_limits(tmp_path):
     _run(tmp_path, "kvpool_limits_driver.cpp", lambda b: b.SOURCES["host_kvpool.cpp"])
+
+
+def test_grids_of_attention(tmp_path):
+    _run(tmp_path, "kvattn_grid_driver.cpp", lambda b: ["-x", "hip", "-fuse-cuid=none", *b.SOURCES["kernels_kvattn.hip"]])
