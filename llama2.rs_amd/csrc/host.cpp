@@ -2437,6 +2437,7 @@ extern "C" int l2_decode_sample(l2_model *m, l2_state *s, int32_t token, int32_t
                                 float min_p, float u, int32_t *next) {
     if (!m || !s || !next) return l2_fail(L2_ERR_ARG, "null argument");
     if (s->m != m) return l2_fail(L2_ERR_ARG, "state belongs to another model");
+    if (m->d.vocab_size > kMaxVocab) return l2_fail(L2_ERR_ARG, "sampling from %d logits (up to 2^19)", m->d.vocab_size);
     const AtWork at_work(m);
     int max_pos = 0;
     L2_TRY(check_tokens(m, &token, &pos, 1, &max_pos));
