@@ -303,10 +303,11 @@ int l2_kvpool_attention(l2_kvpool *p, int layer, const l2_kvbatch *batch, const 
  * first among equals, and weights w = exp((l - max l) / temperature):
  *   top_k:  the first top_k tokens are kept            (off: <= 0)
  *   top_p:  of these, the fewest from the front whose weights reach top_p of the sum of these    (off: >= 1)
- *   min_p:  of these, those with w >= min_p (of the largest weight, which is 1)               (off: <= 0)
+ *   min_p:  of these, those with w >= min_p (of the largest weight, which is 1; above 1: as 1)     (off: <= 0)
  * The first is always kept.  The answer is the first id, in the vocabulary's order, at which the running sum of the kept weights passes u times
- * their sum (Random::sample, src/util.rs:102-113); of a u of 1 or more the last kept, and a u below 0 or NaN is 0.  A temperature of 0 (or below, or NaN) takes the first token.  Weights are whole multiples of 2^-44 and sums of them
- * exact, so a row's answer is the same in every batch and call.  NaN logits count as -infinity; a row with nothing else gets -1.  An infinite
+ * their sum (Random::sample, src/util.rs:102-113); of a u of 1 or more the last kept, and a u below 0 or NaN is 0.  A temperature of 0 (or below, or NaN) takes the first token.  Weights are rounded to whole multiples of 2^-44, and sums of them
+ * exact, so a row's answer is the same in every batch and call; a border between two tokens is off by up to 2^-45 for each token in front of it, and a weight that rounds to zero is never
+ * chosen.  NaN logits count as -infinity; a row with nothing else gets -1.  An infinite
  * logit shares everything with its equals.  vocab up to 2^19, rows up to 2^21.  ids_dev is host-visible or device memory.
  * Enqueued on hip_stream without waiting; allocates nothing; may be captured (after a first call, or l2_kvpool_create, on the device).
  * temperature, top_k, top_p, min_p and u are device arrays [rows]; any of the first four may be NULL: 1, off, off, off. */

@@ -1,8 +1,8 @@
 // One token per row of logits: temperature, top-k, top-p, min-p and a given random number.
 //
 // In falling order of (logit, then id) what every one of the three filters keeps is a prefix, so each is a threshold on that order.  Weights are whole multiples
-// of 2^-44 in 64-bit integers: sums are exact whatever the order atomics come in, so an answer depends on its row alone.  Their rounding moves a border between two tokens
-// by 2^-45 of the largest weight.
+// of 2^-44 in 64-bit integers: sums are exact whatever the order atomics come in, so an answer depends on its row alone.  A weight is off by up to 2^-45 of the largest, so a border
+// between two tokens, which is a sum of n of them, by n times that: 2^-30 of 32000 tokens, 2^-26 of the most.  One that rounds to zero is never chosen.
 //
 // One block of 16 waves per row.  It is bound by the instructions that one CU can issue, not by the 128 KB of a row, so passes are few and short: the largest logit;
 // for top-k, how many logits lie in each of 2048 bins, of those not below the bin that k threads' largest reach, and the tokens of the bin that the k-th is in;
