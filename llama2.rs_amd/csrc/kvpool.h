@@ -83,8 +83,7 @@ __device__ __forceinline__ int page_at(const l2_kvbatch &b, int n_pages, int i, 
     return (uint32_t)p < (uint32_t)n_pages ? p : -1;
 }
 
-// e4m3's codes from a float inside +-448 and back.
-__device__ __forceinline__ uint8_t to_e4m3(float y) { return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false); }
+// What a code of e4m3 stands for.
 __device__ __forceinline__ float from_e4m3(uint8_t c) { return __builtin_amdgcn_cvt_f32_fp8((int)c, 0); }
 
 __device__ __forceinline__ float bf16_float(uint16_t v) { return __builtin_bit_cast(float, (uint32_t)v << 16); }
