@@ -992,15 +992,18 @@ void kv_attention_plan(const KvLayer &l, int kv_type, const l2_kvbatch &b, const
         *splits = *per ? (int)((tiles + *per - 1) / *per) : 1;
     };
     // Where no sequence has more than `most` rows the narrow kernel takes all, cells read once for each 16 rows.  us as narrow and wide, 32 sequences of 2048 positions, 64 heads on
-    // 8: 24, 48 and 64 rows of bf16 on e4m3 53 / 101, 76 / 104 and 88 / 104 (80: 112 / 108), of fp32 on i8 57 / 142, 82 / 148 and 98 / 150, of fp32 on bf16 103 / 260, 138 / 260 and
-    // 167 / 258; of fp16 on fp16, where a block's cells are twice as many and the wide kernel has the least to do, 100 / 104 (32: 101 / 105), 131 / 109 and 173 / 112.
-    const int most = (kv_type > L2_KV_E4M3 && pieces_index(kv_type, a.type) == 0 ? 32 : 64) / group * group;
+    // 8: 24, 48, 64 and 80 rows of bf16 on e4m3 46 / 112, 74 / 106, 86 / 108 and 108 / 111, of fp32 on i8 49 / 125, 79 / 130, 90 / 132 and 112 / 138, of fp32 on bf16, three numbers each, 84 / 206, 131 / 212,
+    // 158 / 215 and 198 / 219.  Over other cells of 16 bits, of which a block reads twice the bytes: 24, 32, 48 and 64 of fp16 on fp16 83 / 99, 83 / 105, 132 / 111 and 156 / 112, of fp32
+    // 84 / 123, 85 / 123, 132 / 129 and 159 / 132.
+    const int most = (kv_type > L2_KV_E4M3 && pieces_index(kv_type, a.type) < 2 ? 32 : 64) / group * group;
     plan->wide = rows * group > most;
     // The one kernel's or the other's alone, where every sequence has that many rows if the call's arrays are full; else they may be some of each.
     if (!plan->wide) plan->narrow_rows = most;
     else plan->narrow_rows = group > kNarrowRows || (b.n_rows - (seqs - 1) * rows) * group > kNarrowRows ? 0 : kNarrowRows / group * group;
     plan->narrow_blocks = (int)std::max<int64_t>((std::min<int64_t>(rows * group, plan->narrow_rows) + kNarrowRows - 1) / kNarrowRows, 1);
     plan->narrow_splits = plan->wide_splits = 1;
+    // Beside chunks, parts as for half of the sequences: where 1, a few, half and all but one of 4, 12 and 32 are chunks, counting a quarter, three quarters or all of them made
+    // such batches up to 8 % quicker or slower, in no order.
     if (plan->narrow_rows)
         parts_of((plan->wide ? (seqs + 1) / 2 : seqs) * l.n_heads * plan->narrow_blocks, 2 * cu_count(), tiles_seen(kv_type <= L2_KV_E4M3 ? 64 : 32, plan->narrow_rows),
                  kNarrowWaves, &plan->narrow_splits, &plan->narrow_per);
