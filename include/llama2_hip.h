@@ -275,7 +275,7 @@ int l2_kvpool_read(l2_kvpool *p, int layer, const l2_kvbatch *batch, void *k_dev
 /* Attention of the rows over one layer: q_dev and out_dev of `type`, [n_rows][n_heads][head_size], n_heads a multiple of the pool's (query
  * head h reads kv head h / (n_heads / n_kv_heads)); out may be q, with its stride.  The row of position pos sees the positions t <= pos that have a page, with a window > 0
  * only those of the last `window` (t > pos - window) and of the first `sinks`.  out = sum over t of softmax(scale * q.k_t) v_t;
- * zeros where nothing is seen.  Keys and values come from the pool, those of the rows included (l2_kvpool_write first).  Scores, statistics and sums
+ * zeros where nothing is seen, or no score that is not -infinity.  Keys and values come from the pool, those of the rows included (l2_kvpool_write first).  Scores, statistics and sums
  * are fp32; q of 16 bits enters the matrix cores as it is, fp32 q and all weights of the softmax as several 16-bit numbers: to within 2^-22
  * (over L2_KV_BF16 2^-24, for 16-bit rows 2^-16), a weight also, but over L2_KV_BF16, to no less than 2^-32 of the largest, in 8 bits each times the scale of its values.  What is not seen has no influence, NaN and infinities included.
  * A value that is not finite makes its dimension the sum of those; a row that sees a key with infinities may be NaN where the formula is not.  Scores are good

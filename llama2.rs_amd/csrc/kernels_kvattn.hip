@@ -192,8 +192,8 @@ struct Parts {
 // Sequences of few query rows per kv head (new tokens x query heads of the group).  A block has 16 rows of one sequence and kv head and part of the positions, its
 // four waves tiles of 64 positions (32 of 16-bit cells) in turn, straight from memory into registers: 8 KB of keys and 8 KB of values, the next tile's keys
 // asked for once this one's scores are there and its values once this one's are summed.  LDS only joins the waves: a row of V^T or K is read by one wave alone.
-// Bound by memory where the launch fills the chip: 32 sequences' next tokens, 64 heads on 8, up to 4096 positions in e4m3, 48 us (39 at a large copy's rate);
-// one behind 60001 positions of 32 heads in i8, 102 us (4.9 TB/s; at a copy's rate 108).  One behind 500 takes 11 us: two launches, and in each two or three trips
+// Bound by memory where the launch fills the chip: 32 sequences' next tokens, 64 heads on 8, up to 4096 positions in e4m3, 49 us (29 at the 6.3 TB/s
+// of launches that only read); one behind 60001 positions of 32 heads in i8, 103 us (80).  One behind 500 takes 11 us: two launches, and in each two or three trips
 // to memory that wait for one another.
 template <int KV, int NQ, int D>
 __global__ __launch_bounds__(64 * kNarrowWaves, 2) void kv_narrow_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, Cut cut) {
@@ -576,9 +576,9 @@ __device__ __forceinline__ void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n
 // with two places for keys and three for the rest, tile i + 1 may be written from step 2 i on, and is there before 2 i + 2.
 //
 // Of heads of 128, a wave's products of a tile are 512 clocks of its matrix core per number that q is made of, and as many per number of a weight: 1536 of 16-bit rows.  Each score
-// and weight of 8-bit cells is multiplied by a scale, and conversion is the vector ALUs' too.  512 rows of 64 heads on 8 behind 7488 positions in i8: 207 us, 630 TFLOP/s of what
-// one number each would take (a large library product in fp16: 1170); two prompts of 4096 and 2542, 32 heads, window 1024, bf16: 193 us, 490 TFLOP/s, of which a quarter is the last of four rounds of
-// blocks.  Weights in one number took 168 and 162.  What did not pay: one conversion spread between the products
+// and weight of 8-bit cells is multiplied by a scale, and conversion is the vector ALUs' too.  512 rows of 64 heads on 8 behind 7488 positions in i8: 206 us, 630 TFLOP/s of what
+// one number each would take (a large library product in fp16: 1170); two prompts of 4096 and 2542, 32 heads, window 1024, bf16: 204 us, 464 TFLOP/s, of which a quarter is the last of four rounds of
+// blocks.  Weights in one number took 171 and 171.  What did not pay: one conversion spread between the products
 // (+9 %), the values' wait half a tile later, scales as float4 from LDS (16 reads a tile; they now are two registers, broadcast in rows of lanes).
 template <int KV, int NQ, int D>
 __global__ __launch_bounds__(kWideThreads, 2) void kv_wide_kernel(KvLayer l, l2_kvbatch b, KvAttention a, Parts parts, Cut cut) {
