@@ -6,7 +6,7 @@
 // nothing is transposed here.  Codes of 8 bits become 16-bit floats exactly (fp16).  Scales of keys multiply the scores, those of values the weights.
 //
 // Weights enter the second product in 16 bits, times a factor that cancels in the quotient with their sum: p_t = exp2(s_t - off).  `off` follows the largest s_t + log2 of the
-// scale of v_t, so that p_t * (scale of v_t) is what is bounded, by 2^15 for fp16, and the largest of these is 2^7 or more (over bf16, of values up to 2^127, 1 and 2^-8): off goes to 7 below it, and
+// scale of v_t, so that p_t * (scale of v_t) is what is bounded, by 2^15 for fp16, and the largest of these is 2^7 or more (over bf16 2^-16 and 2^-24, whose small numbers are as good: sums over 2^16 positions are finite, whatever the values): off goes to 7 below it, and
 // is left where it is until it lies more than 8 higher, so that sums are seldom rescaled (a tile of 32 rows would have a new maximum among them nearly always).  The largest s
 // with the largest scale of a tile, which a product of less weight may have, only says whether that may be so: where it may, the positions are gone over one by one.
 // Weights, times scales, are two fp16 numbers each (to within 2^-22, and no less than 2^-32 of the largest) or, over a pool in bf16, two of bf16 (2^-16) for rows of 16 bits and three for
@@ -33,7 +33,7 @@ constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLeastE = -67.f; // rows whose values are held at all have scales from 2^-67
 constexpr float kSlack = 8.f;
-constexpr float base_of(int kv_type) { return kv_type == L2_KV_BF16 ? -8.f : 7.f; }
+constexpr float base_of(int kv_type) { return kv_type == L2_KV_BF16 ? -24.f : 7.f; }
 
 // `off` behind a tile whose largest score times its factor, with the scale of its values, is `top`, and the factor of the sums so far.
 template <int KV>

@@ -26,8 +26,8 @@ def _weight(kv, t):
 
 def _bound(kv, t, q, k, v, scale, want):
     """Element by element.  A score's products and their sum are off by a rounding each, its factors by four; the quotient by twice what the
-    score is off, by its weight's numbers, the exponential (2^-22) and the n roundings of a sum; a weight is known to no less than
-    2^-32 of the largest (times the scale of its values, which is 2^-6 of the row's largest or less)."""
+    score is off, by its weight's numbers, the exponential (2^-22) and the n roundings of a sum; over fp16 and 8 bits a weight is known to no less than
+    2^-32 of the largest (in 8 bits times the scale of its values, which is 2^-6 of the row's largest or less)."""
     n, D = v.shape
     most = float((np.abs(k.astype(np.float64)) @ np.abs(q.astype(np.float64))).max() * scale)
     score = most * ((D + 4) * 2.0 ** -24 + (2.0 ** -21 if t == F32 else 0.0))
@@ -36,9 +36,9 @@ def _bound(kv, t, q, k, v, scale, want):
     p /= p.sum()
     size = p @ np.abs(v.astype(np.float64))
     off = size * (2 * score + _weight(kv, t) + 2.0 ** -21 + (n + 64) * 2.0 ** -24)
-    if kv in ("f16", "bf16"):
+    if kv == "f16":
         off = off + 2.0 ** -32 * p.max() * np.abs(v).sum(0)
-    else:
+    elif kv != "bf16":
         a = np.maximum(np.abs(v).max(1), 2.0 ** -60).astype(np.float64)
         off = off + 2.0 ** -32 * (p * a).max() * (np.abs(v) / a[:, None]).sum(0)
     return 1.01 * off + (np.abs(want) + off) * plain.HALF_STEP[t] + TINY[t]
@@ -169,6 +169,18 @@ def test_values_of_1e36_in_bf16(dev, t, lengths, rows):
     v = (2.0 ** 117 * rng.standard_normal((sum(lengths), 1, 64))).astype(np.float32)
     c, _ = _cache(dev, "bf16", t, lengths, None, v)
     q = rng.standard_normal((sum(rows), 2, 64)).astype(np.float32)
+    _check(c, "bf16", t, c.attend(q, rows, t, 2), q, rows, 2)
+    c.close()
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("lengths,rows", [([1500, 300], [1, 3]), ([700], [100])])
+def test_the_largest_values_of_bf16(dev, t, lengths, rows):
+    """Values of one sign near the type's largest: their mean is one of them, though a sum of two is none."""
+    rng = np.random.default_rng(8)
+    v = (3e38 * (1 - 0.1 * rng.random((sum(lengths), 1, 64)))).astype(np.float32)
+    c, _ = _cache(dev, "bf16", t, lengths, None, v)
+    q = (0.01 * rng.standard_normal((sum(rows), 2, 64))).astype(np.float32)  # weights much alike
     _check(c, "bf16", t, c.attend(q, rows, t, 2), q, rows, 2)
     c.close()
 
